@@ -826,6 +826,125 @@ SUBSPEC_API int subspec_lm_head_verify_scratch_bytes(int32_t batch, int32_t max_
                                                      int32_t vocab, size_t* bytes);
 SUBSPEC_API int subspec_lm_head_verify(const subspec_lm_head_verify_args* args, subspec_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Chunks of new tokens over the paged cache: prompts, and whatever a request
+ * brings at once, many requests to a call, their tokens packed one request
+ * behind the other (token t of the call belongs to the request b with
+ * q_indptr[b] <= t < q_indptr[b + 1]).  Four steps: the plan (once a step),
+ * then per layer the append and the attention.
+ *
+ * Beside subspec_pages_update / subspec_kv_append_paged /
+ * subspec_tree_attention_paged, which serve trees of one size per request:
+ * they cover the reference's FlashInfer calls around a prompt
+ *   - KvCachePool.allocate, RequestKvCache.increment, getKvCacheBatchPosition
+ *       specdecodes/models/utils/flashinfer/cache_manager.py:66-80, 237-414
+ *   - append_paged_kv_cache and BatchPrefillWithPagedKVCacheWrapper.run with
+ *     causal=True
+ *       specdecodes/models/utils/flashinfer/attention_wrapper.py:104-151, 234-316
+ * ---------------------------------------------------------------------- */
+
+/* Block tables and slot maps from request lengths.  State as for
+ * subspec_pages_update.  Per request: base = set_len ? set_len[b] : kv_len[b] rows are kept, pages behind them go
+ * back to the pool (their page_table entries become -1), kv_len[b] = base + n_new[b], and missing pages are the
+ * lowest free ones, requests in batch order, all releases first.  q_indptr = the exclusive sum of n_new.  Token t:
+ * batch_indices[t] = b, positions[t] = base + t - q_indptr[b], slot_map[t] = page * page_len + row.  The entries
+ * from the last token to max_tokens become batch -1, position 0, slot -1, which the append skips.  Set in
+ * dev_status: SUBSPEC_DEV_BAD_COUNT for a negative length (read as 0) or more than max_tokens tokens (the rest gets
+ * no entry), SUBSPEC_DEV_BAD_PAGE where pages or a row of page_table run out (those tokens get slot -1; kv_len stops
+ * at the capacity of the page_table row). */
+typedef struct subspec_chunk_plan_args {
+  uint32_t struct_size;
+  int32_t batch;
+  int32_t num_pages;
+  int32_t page_len;
+  int32_t pages_per_seq;
+  int32_t max_tokens;        /* entries of slot_map / positions / batch_indices */
+  uint32_t* free_mask;       /* [(num_pages + 31) / 32] */
+  int32_t* page_table;       /* [batch, pages_per_seq] */
+  int32_t* n_pages;          /* [batch] */
+  int32_t* kv_len;           /* [batch] */
+  int32_t* kv_last_page_len; /* [batch] or NULL */
+  const int32_t* set_len;    /* [batch] or NULL */
+  const int32_t* n_new;      /* [batch] */
+  int32_t* q_indptr;         /* [batch + 1] */
+  int64_t* slot_map;         /* [max_tokens] */
+  int32_t* positions;        /* [max_tokens] */
+  int32_t* batch_indices;    /* [max_tokens] */
+  uint32_t* dev_status;
+} subspec_chunk_plan_args;
+
+SUBSPEC_API int subspec_chunk_plan(const subspec_chunk_plan_args* args, subspec_stream_t stream);
+
+/* K / V rows of packed tokens to their slots of one layer: row t goes to row slot_map[t] % page_len of page
+ * slot_map[t] / page_len.  A negative slot is skipped, one past the pool is skipped and sets SUBSPEC_DEV_BAD_INDEX.
+ * The slots of a call are distinct.  Strides in elements, multiples of 8; head_dim a multiple of 8. */
+typedef struct subspec_kv_append_slots_args {
+  uint32_t struct_size;
+  int32_t tokens;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t layer;
+  int32_t layers;
+  int32_t num_pages;
+  int32_t page_len;
+  void* pool;
+  const void* k;
+  const void* v;
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  const int64_t* slot_map; /* [tokens] */
+  uint32_t* dev_status;
+} subspec_kv_append_slots_args;
+
+SUBSPEC_API int subspec_kv_append_slots(const subspec_kv_append_slots_args* args, subspec_stream_t stream);
+
+/* Attention of packed tokens over their requests' cache rows.  kv_len[b] counts the rows INCLUDING the request's new
+ * ones (append first): with n = q_indptr[b + 1] - q_indptr[b], its i-th token sits at row p = kv_len[b] - n + i and
+ * sees rows 0 .. p; with window > 0 only those of rows p - window + 1 .. p and 0 .. sinks - 1.  Rows that no token
+ * of the request can see are not read, so a request may have given back the pages that left its window
+ * (page_table entry -1).  A token that sees nothing (kv_len[b] < n, which also sets SUBSPEC_DEV_BAD_COUNT) gets
+ * zeros; rows of `out` behind the last request's are left as they were.  What a row does not see has no influence on
+ * it, infinities and NaN included.
+ * q / out [tokens, num_q_heads, head_dim] in the pool's type with element strides; query head h reads KV head
+ * h / (num_q_heads / num_kv_heads); head_dim 64 or 128.  Softmax in fp32.  max_q_len: no request of the call brings
+ * more tokens (a request that does sets SUBSPEC_DEV_BAD_COUNT and its last tokens get no output).
+ * kv_splits: cache ranges for several CTAs per query tile, 0 = chosen from the sizes.  scratch:
+ * subspec_chunk_attention_scratch_bytes of the same arguments, 16-byte aligned, owned by the call until the stream has
+ * passed it; need not be initialised. */
+typedef struct subspec_chunk_attn_args {
+  uint32_t struct_size;
+  int32_t batch;
+  int32_t tokens;    /* rows of q and out */
+  int32_t max_q_len; /* most tokens of one request */
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t layer;
+  int32_t layers;
+  int32_t num_pages;
+  int32_t page_len;
+  int32_t pages_per_seq;
+  int32_t dtype;     /* SUBSPEC_BF16 or SUBSPEC_F16: pool, q and out alike */
+  int32_t window;    /* 0: none */
+  int32_t sinks;
+  int32_t kv_splits;
+  const void* pool;
+  const int32_t* page_table; /* [batch, pages_per_seq] */
+  const int32_t* kv_len;     /* [batch] */
+  const int32_t* q_indptr;   /* [batch + 1], ascending from 0 */
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  void* out;
+  int64_t o_token_stride, o_head_stride;
+  double sm_scale;
+  uint32_t* dev_status;
+  void* scratch;
+  size_t scratch_bytes;
+} subspec_chunk_attn_args;
+
+SUBSPEC_API int subspec_chunk_attention_scratch_bytes(const subspec_chunk_attn_args* args, size_t* bytes);
+SUBSPEC_API int subspec_chunk_attention_paged(const subspec_chunk_attn_args* args, subspec_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

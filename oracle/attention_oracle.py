@@ -43,3 +43,27 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: torc
         s = s.masked_fill(~mask, float("-inf"))
         out[:, h] = torch.softmax(s, dim=-1) @ vd[:, h // G]
     return out
+
+
+def chunk_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int = 0, sinks: int = 0, sm_scale=None):
+    """Causal attention of the last rows of a request: q [n, HQ, D], its cache rows k / v [kv_len, HKV, D], query i at
+    row kv_len - n + i; window > 0: rows p - window + 1 .. p and 0 .. sinks - 1 only.  A row is the sum over what it
+    sees and nothing else (what lies in hidden rows cannot reach it).  Returns (out, sum of weight * |v|) in float64:
+    the second bounds what a relative error of the weights does to the first."""
+    n, HQ, D = q.shape
+    kv_len, HKV = k.shape[0], k.shape[1]
+    G = HQ // HKV
+    scale = 1.0 / math.sqrt(D) if sm_scale is None else sm_scale
+    out, mag = torch.zeros(n, HQ, D, dtype=torch.float64), torch.zeros(n, HQ, D, dtype=torch.float64)
+    qd, kd, vd = q.double(), k.double().repeat_interleave(G, 1), v.double().repeat_interleave(G, 1)
+    for i in range(n):
+        p = kv_len - n + i
+        if p < 0:
+            continue
+        rows = torch.arange(p + 1)
+        if window:
+            rows = rows[(rows > p - window) | (rows < sinks)]
+        w = torch.softmax(torch.einsum("hd,jhd->hj", qd[i], kd[rows]) * scale, -1)
+        out[i] = torch.einsum("hj,jhd->hd", w, vd[rows])
+        mag[i] = torch.einsum("hj,jhd->hd", w, vd[rows].abs())
+    return out, mag

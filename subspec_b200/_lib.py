@@ -199,6 +199,42 @@ class KvAppendArgs(C.Structure):
     ]
 
 
+class ChunkPlanArgs(C.Structure):
+    """Mirror of `subspec_chunk_plan_args`."""
+
+    _fields_ = [
+        ("struct_size", _u32), ("batch", _i32), ("num_pages", _i32), ("page_len", _i32), ("pages_per_seq", _i32),
+        ("max_tokens", _i32), ("free_mask", _vp), ("page_table", _vp), ("n_pages", _vp), ("kv_len", _vp),
+        ("kv_last_page_len", _vp), ("set_len", _vp), ("n_new", _vp), ("q_indptr", _vp), ("slot_map", _vp),
+        ("positions", _vp), ("batch_indices", _vp), ("dev_status", _vp),
+    ]
+
+
+class KvAppendSlotsArgs(C.Structure):
+    """Mirror of `subspec_kv_append_slots_args`."""
+
+    _fields_ = [
+        ("struct_size", _u32), ("tokens", _i32), ("num_kv_heads", _i32), ("head_dim", _i32), ("layer", _i32),
+        ("layers", _i32), ("num_pages", _i32), ("page_len", _i32), ("pool", _vp), ("k", _vp), ("v", _vp),
+        ("k_token_stride", _i64), ("k_head_stride", _i64), ("v_token_stride", _i64), ("v_head_stride", _i64),
+        ("slot_map", _vp), ("dev_status", _vp),
+    ]
+
+
+class ChunkAttnArgs(C.Structure):
+    """Mirror of `subspec_chunk_attn_args`."""
+
+    _fields_ = [
+        ("struct_size", _u32), ("batch", _i32), ("tokens", _i32), ("max_q_len", _i32), ("num_q_heads", _i32),
+        ("num_kv_heads", _i32), ("head_dim", _i32), ("layer", _i32), ("layers", _i32), ("num_pages", _i32),
+        ("page_len", _i32), ("pages_per_seq", _i32), ("dtype", _i32), ("window", _i32), ("sinks", _i32),
+        ("kv_splits", _i32), ("pool", _vp), ("page_table", _vp), ("kv_len", _vp), ("q_indptr", _vp), ("q", _vp),
+        ("q_token_stride", _i64), ("q_head_stride", _i64), ("out", _vp), ("o_token_stride", _i64),
+        ("o_head_stride", _i64), ("sm_scale", _f64), ("dev_status", _vp), ("scratch", _vp),
+        ("scratch_bytes", C.c_size_t),
+    ]
+
+
 W4A16_MAX_GROUP = 4
 
 
@@ -230,6 +266,10 @@ SYMBOLS = {
     "subspec_pages_update": (C.c_int, [C.POINTER(PagesArgs), _vp]),
     "subspec_tree_attention_paged": (C.c_int, [C.POINTER(TreeAttnArgs), _vp]),
     "subspec_kv_append_paged": (C.c_int, [C.POINTER(KvAppendArgs), _vp]),
+    "subspec_chunk_plan": (C.c_int, [C.POINTER(ChunkPlanArgs), _vp]),
+    "subspec_kv_append_slots": (C.c_int, [C.POINTER(KvAppendSlotsArgs), _vp]),
+    "subspec_chunk_attention_scratch_bytes": (C.c_int, [C.POINTER(ChunkAttnArgs), C.POINTER(C.c_size_t)]),
+    "subspec_chunk_attention_paged": (C.c_int, [C.POINTER(ChunkAttnArgs), _vp]),
     "subspec_tree_prune_depth": (C.c_int, [C.POINTER(TreePruneDepthArgs), _vp]),
     "subspec_w4a16_packed_bytes": (C.c_int, [_i32, _i32, C.POINTER(C.c_size_t)]),
     "subspec_w4a16_pack": (C.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _vp]),

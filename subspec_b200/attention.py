@@ -196,3 +196,138 @@ def tree_attention_static(q: torch.Tensor, key_cache: torch.Tensor, value_cache:
                "subspec_tree_attention_paged")
     del scratch
     return out
+
+
+def _aligned(t: torch.Tensor) -> bool:
+    """Whether every row of the last axis can be read 16 bytes at a time."""
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1])
+
+
+def _check_pool(pool: torch.Tensor, layer: int) -> None:
+    if pool.dim() != 6 or pool.shape[2] != 2 or not pool.is_contiguous() or \
+            pool.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("pool must be a contiguous bf16 or fp16 [layers, pages, 2, page_len, kv_heads, head_dim] tensor")
+    if not 0 <= int(layer) < pool.shape[0]:
+        raise ValueError("layer outside the pool")
+
+
+@torch.no_grad()
+def append_paged_kv_slots(pool: torch.Tensor, layer: int, k: torch.Tensor, v: torch.Tensor, *, slot_map: torch.Tensor,
+                          status: Optional[torch.Tensor] = None) -> None:
+    """k, v [tokens, kv_heads, head_dim] of packed requests -> rows `slot_map[t]` of layer `layer`.
+
+    `slot_map` int64 [>= tokens] as `DevicePagePool.plan_chunks` leaves it: page * page_len + row, all different;
+    negative ones are skipped (a padded batch), one past the pool sets `status`.  k and v may be slices of a fused
+    projection."""
+    _check_pool(pool, layer)
+    L, P, _, page_len, H, D = (int(x) for x in pool.shape)
+    if k.dim() != 3 or k.shape != v.shape or tuple(k.shape[1:]) != (H, D) or k.dtype != pool.dtype or \
+            v.dtype != pool.dtype or k.device != pool.device or v.device != pool.device:
+        raise ValueError("k and v must be [tokens, kv_heads, head_dim] tensors of the pool's type on its device")
+    T = int(k.shape[0])
+    if slot_map.dtype != torch.int64 or slot_map.device != pool.device or slot_map.dim() != 1 or \
+            slot_map.numel() < T or not slot_map.is_contiguous():
+        raise ValueError("slot_map must be a contiguous int64 tensor on the pool's device with an entry per token")
+    if D % 8:
+        raise ValueError("head_dim must be a multiple of 8")
+    if T == 0:
+        return
+    k, v = (x if _aligned(x) else x.clone(memory_format=torch.contiguous_format) for x in (k, v))
+    a = _lib.KvAppendSlotsArgs()
+    a.struct_size = C.sizeof(_lib.KvAppendSlotsArgs)
+    a.tokens, a.num_kv_heads, a.head_dim = T, H, D
+    a.layer, a.layers, a.num_pages, a.page_len = int(layer), L, P, page_len
+    a.pool, a.k, a.v, a.slot_map = pool.data_ptr(), k.data_ptr(), v.data_ptr(), slot_map.data_ptr()
+    a.k_token_stride, a.k_head_stride = int(k.stride(0)), int(k.stride(1))
+    a.v_token_stride, a.v_head_stride = int(v.stride(0)), int(v.stride(1))
+    a.dev_status = 0 if status is None else status.data_ptr()
+    with torch.cuda.device(pool.device):
+        stream = torch.cuda.current_stream(pool.device).cuda_stream
+        _lib.check(_lib.lib().subspec_kv_append_slots(C.byref(a), C.c_void_p(stream)), "subspec_kv_append_slots")
+
+
+def _chunk_attention(what: str, q, pool, layer, page_table, kv_len, q_indptr, max_q_len, window, sinks, sm_scale, status,
+                     out, kv_splits) -> torch.Tensor:
+    _check_pool(pool, layer)
+    L, P, _, page_len, H, D = (int(x) for x in pool.shape)
+    if q.dim() != 3 or q.dtype != pool.dtype or q.device != pool.device or int(q.shape[2]) != D or D not in (64, 128):
+        raise ValueError("q must be [tokens, q_heads, head_dim] of the pool's type and head_dim (64 or 128) on its device")
+    T, HQ = int(q.shape[0]), int(q.shape[1])
+    if HQ < 1 or HQ % H:
+        raise ValueError("q_heads must be a multiple of the pool's kv_heads")
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous() or \
+            page_table.device != pool.device:
+        raise ValueError("page_table must be a contiguous int32 [batch, pages_per_seq] tensor on the pool's device")
+    B = int(page_table.shape[0])
+    if out is None:
+        out = torch.empty(T, HQ, D, dtype=q.dtype, device=q.device)
+    elif out.dtype != q.dtype or out.shape != q.shape or out.device != q.device or not (T == 0 or _aligned(out)):
+        raise ValueError("out must be a tensor of q's type and shape on q's device, its rows 16-byte aligned")
+    if max_q_len is None:
+        max_q_len = T
+    elif not 0 <= int(max_q_len):
+        raise ValueError("max_q_len must not be negative")
+    a = _lib.ChunkAttnArgs()
+    a.struct_size = C.sizeof(_lib.ChunkAttnArgs)
+    a.batch, a.tokens, a.max_q_len, a.num_q_heads, a.num_kv_heads, a.head_dim = B, T, min(int(max_q_len), T), HQ, H, D
+    a.layer, a.layers, a.num_pages, a.page_len = int(layer), L, P, page_len
+    a.pages_per_seq = int(page_table.shape[1])
+    a.dtype = _lib.BF16 if q.dtype == torch.bfloat16 else _lib.F16
+    a.window, a.sinks = window, sinks
+    a.kv_splits = 0 if kv_splits is None else int(kv_splits)
+    if kv_splits is not None and not 1 <= int(kv_splits) <= 1024:
+        raise ValueError("kv_splits must be between 1 and 1024")
+    a.pool, a.page_table = pool.data_ptr(), page_table.data_ptr()
+    a.kv_len, a.q_indptr = _i32(kv_len, pool.device, B, "kv_len"), _i32(q_indptr, pool.device, B + 1, "q_indptr")
+    if T == 0 or B == 0:
+        return out
+    if not _aligned(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    a.q, a.q_token_stride, a.q_head_stride = q.data_ptr(), int(q.stride(0)), int(q.stride(1))
+    a.out, a.o_token_stride, a.o_head_stride = out.data_ptr(), int(out.stride(0)), int(out.stride(1))
+    a.sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(D)
+    a.dev_status = 0 if status is None else status.data_ptr()
+    with torch.cuda.device(pool.device):
+        need = C.c_size_t(0)
+        _lib.check(_lib.lib().subspec_chunk_attention_scratch_bytes(C.byref(a), C.byref(need)), what)
+        scratch = torch.empty(need.value, dtype=torch.uint8, device=pool.device) if need.value else None
+        if scratch is not None:
+            a.scratch, a.scratch_bytes = scratch.data_ptr(), need.value
+        stream = torch.cuda.current_stream(pool.device).cuda_stream
+        _lib.check(_lib.lib().subspec_chunk_attention_paged(C.byref(a), C.c_void_p(stream)), what)
+    return out
+
+
+@torch.no_grad()
+def chunk_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, page_table: torch.Tensor,
+                          kv_len: torch.Tensor, q_indptr: torch.Tensor, max_q_len: Optional[int] = None,
+                          sm_scale: Optional[float] = None, status: Optional[torch.Tensor] = None,
+                          out: Optional[torch.Tensor] = None, kv_splits: Optional[int] = None) -> torch.Tensor:
+    """Causal attention of packed chunks over the paged cache: q [tokens, q_heads, head_dim (64 or 128)] -> the same
+    shape (into `out` when given: a captured graph needs a buffer that outlives the capture).
+
+    Request b's tokens are q_indptr[b] .. q_indptr[b + 1] - 1 of q, the last rows of its cache: kv_len[b] counts them in
+    (append first), and each sees the rows up to its own.  One token (a decode step) to whole prompts, mixed at will.
+    `max_q_len`: no request brings more (default: all the tokens) -- give it where it is known, the kernels for a few
+    rows per request are chosen by it.  Rows of the output behind q_indptr[-1] are left as they were; what a token does
+    not see has no influence on it, infinities and NaN included.  What `DevicePagePool.plan_chunks` returned fits as
+    it is: chunk_attention_paged(q, pool, layer, page_table=plan.page_table, kv_len=plan.kv_len, q_indptr=plan.q_indptr)."""
+    return _chunk_attention("chunk_attention_paged", q, pool, layer, page_table, kv_len, q_indptr, max_q_len, 0, 0,
+                            sm_scale, status, out, kv_splits)
+
+
+@torch.no_grad()
+def window_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, page_table: torch.Tensor,
+                           kv_len: torch.Tensor, q_indptr: torch.Tensor, window: int, sinks: int = 0,
+                           max_q_len: Optional[int] = None, sm_scale: Optional[float] = None,
+                           status: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                           kv_splits: Optional[int] = None) -> torch.Tensor:
+    """`chunk_attention_paged` under a sliding window: a token at row p sees the `window` rows up to its own and the
+    first `sinks` rows of the request.  Pages that lie outside every token's view are not read: they may have been given
+    back (page_table entry -1)."""
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError("window must be at least 1 and sinks not negative")
+    cap = int(page_table.shape[-1]) * int(pool.shape[3]) if page_table.dim() == 2 and pool.dim() == 6 else window
+    return _chunk_attention("window_attention_paged", q, pool, layer, page_table, kv_len, q_indptr, max_q_len,
+                            max(1, min(window, cap)), min(sinks, cap), sm_scale, status, out, kv_splits)

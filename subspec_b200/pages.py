@@ -11,6 +11,7 @@ flattened page-table tensors of the attention plan rebuilt -- nothing is read ba
 from __future__ import annotations
 
 import ctypes as C
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -19,6 +20,19 @@ from . import _lib
 from .kv_cache import KvCacheBatchPosition
 
 _MODES = {"prefill": _lib.PAGES_PREFILL, "decode": _lib.PAGES_DECODE, "tree": _lib.PAGES_TREE}
+
+
+@dataclass
+class ChunkPlan:
+    """Where the new tokens of a step go, packed one request behind the other (the pool's own buffers: the next
+    `plan_chunks` or `update` overwrites them)."""
+
+    q_indptr: torch.Tensor       # int32 [batch + 1]: tokens of request b are q_indptr[b] .. q_indptr[b + 1] - 1
+    slot_map: torch.Tensor       # int64 [max_append]: page * page_len + row; -1: no place, or behind the last token
+    positions: torch.Tensor      # int32 [max_append]: row of the token in its request's cache
+    batch_indices: torch.Tensor  # int32 [max_append]: request of the token; -1 behind the last one
+    page_table: torch.Tensor     # int32 [batch, pages_per_seq], the live table
+    kv_len: torch.Tensor         # int32 [batch], the new tokens' rows counted in
 
 
 class DevicePagePool:
@@ -44,6 +58,7 @@ class DevicePagePool:
         self.max_append = int(max_append)
         self.batch_indices = torch.zeros(max(1, self.max_append), **i32)
         self.positions = torch.zeros(max(1, self.max_append), **i32)
+        self.slot_map = torch.full((max(1, self.max_append),), -1, dtype=torch.int64, device=dev)
         self.status = torch.zeros(1, **i32)
 
     @torch.no_grad()
@@ -82,6 +97,42 @@ class DevicePagePool:
         return KvCacheBatchPosition(seq_indptr=self.seq_indptr, kv_page_indptr=self.kv_page_indptr,
                                     kv_page_indices=self.kv_page_indices, kv_last_page_len=self.kv_last_page_len,
                                     batch_indices=self.batch_indices, positions=self.positions)
+
+    @torch.no_grad()
+    def plan_chunks(self, n_new: torch.Tensor, *, set_len: Optional[torch.Tensor] = None) -> ChunkPlan:
+        """Block tables and slot maps of a step in which request b brings `n_new[b]` tokens (0 allowed), on the current
+        stream (no synchronisation): `getKvCacheBatchPosition` for chunks of any lengths.
+
+        `set_len[b]` (default `kv_len[b]`) rows are kept, the pages behind them go back to the pool and their entries
+        of `page_table` become -1; then kv_len[b] = set_len[b] + n_new[b], missing pages are the lowest free ones,
+        requests in batch order.  The plan's `slot_map` goes to `append_paged_kv_slots`, its `q_indptr`, `page_table`
+        and `kv_len` to `chunk_attention_paged` / `window_attention_paged`; `max_append` of the constructor bounds the
+        tokens of a step.  Running out of pages or of `max_append` is reported by `check_status`."""
+        if self.max_append < 1:
+            raise ValueError("plan_chunks needs a pool made with max_append: the most tokens a step brings")
+        a = _lib.ChunkPlanArgs()
+        a.struct_size = C.sizeof(_lib.ChunkPlanArgs)
+        a.batch, a.num_pages, a.page_len, a.pages_per_seq = self.batch, self.num_pages, self.page_len, self.pages_per_seq
+        a.max_tokens = self.max_append
+        keep = []
+        for name, t in (("n_new", n_new), ("set_len", set_len)):
+            if t is None:
+                continue
+            if t.is_floating_point() or t.numel() != self.batch:
+                raise ValueError(f"{name} must hold one whole number per request")
+            t = t.to(self.device, torch.int32).contiguous()
+            keep.append(t)
+            setattr(a, name, t.data_ptr())
+        a.free_mask, a.page_table, a.n_pages = self.free_mask.data_ptr(), self.page_table.data_ptr(), self.n_pages.data_ptr()
+        a.kv_len, a.kv_last_page_len = self.kv_len.data_ptr(), self.kv_last_page_len.data_ptr()
+        a.q_indptr, a.slot_map = self.seq_indptr.data_ptr(), self.slot_map.data_ptr()
+        a.positions, a.batch_indices = self.positions.data_ptr(), self.batch_indices.data_ptr()
+        a.dev_status = self.status.data_ptr()
+        with torch.cuda.device(self.device):
+            stream = torch.cuda.current_stream(self.device).cuda_stream
+            _lib.check(_lib.lib().subspec_chunk_plan(C.byref(a), C.c_void_p(stream)), "subspec_chunk_plan")
+        return ChunkPlan(q_indptr=self.seq_indptr, slot_map=self.slot_map, positions=self.positions,
+                         batch_indices=self.batch_indices, page_table=self.page_table, kv_len=self.kv_len)
 
     def num_free_pages(self) -> int:
         """Synchronises: free pages of the pool (bits of the mask inside the pool)."""

@@ -113,7 +113,7 @@ class SpeculativeLoopBatch(SpeculativeStepBatch):
 
     def __init__(self, batch: int, max_nodes: int, device, *, kv_layers: int, kv_heads: int = 4, head_dim: int = 128,
                  page_len: int = 16, pages_per_seq: int, num_pages: Optional[int] = None,
-                 kv_dtype: torch.dtype = torch.bfloat16, init_len=1):
+                 kv_dtype: torch.dtype = torch.bfloat16, init_len=1, max_chunk_tokens: int = 0):
         from .pages import DevicePagePool
         from .postverify import PostVerifyState
 
@@ -122,12 +122,24 @@ class SpeculativeLoopBatch(SpeculativeStepBatch):
         self.pool = torch.empty(kv_layers, num_pages, 2, page_len, kv_heads, head_dim, dtype=kv_dtype,
                                 device=self.device)
         self.pages = DevicePagePool(batch, num_pages, page_len, pages_per_seq, self.device,
-                                    max_append=batch * max_nodes)
+                                    max_append=max(batch * max_nodes, int(max_chunk_tokens)))
         self.page_table = self.pages.page_table  # the compaction kernel reads the live table
         init = torch.as_tensor(init_len, dtype=torch.int32).expand(batch).contiguous()
         self.pages.update(set_len=init, mode="prefill")
         self.state = PostVerifyState(batch, 4 * (max_nodes + 1), self.device, kv_len=init)
         self.tree_tokens = 0
+
+    def begin_chunk(self, n_new: torch.Tensor):
+        """Requests take in chunks of tokens outside the tree step -- prompts, or the next part of one: `n_new[b]` new
+        rows for request b (0: none), in place behind its rows.  Returns the `ChunkPlan` whose slot map
+        `append_paged_kv_slots` takes and whose lengths `chunk_attention_paged` takes.  The new rows count as committed,
+        so call it between steps, for requests whose reorder is not put off (`state.beam_len[b] == 0`): with rows of an
+        earlier tree still waiting, the call keeps to the committed rows and would cut those off.  No synchronisation.
+        The loop needs `max_append >= n_new.sum()`: the constructor's `max_chunk_tokens`."""
+        st = self.state
+        plan = self.pages.plan_chunks(n_new, set_len=st.kv_len)
+        st.kv_len.copy_(plan.kv_len)
+        return plan
 
     def begin_step(self, tree_tokens: int):
         """Room for the next tree in every request's cache (RequestKvCache.increment); returns the page-table
