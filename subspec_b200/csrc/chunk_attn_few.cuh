@@ -1,0 +1,15 @@
+// Entry to the kernel for requests with few rows (chunk_attn_few.cu).
+#pragma once
+
+#include "chunk_attn.cuh"
+
+namespace subspec {
+
+// Tensor maps of a layer's K and V rows for tiles (of a CTA or a warp) of `rows` cache rows; sets ka.box_rows.
+void chunk_tensor_maps(ChunkArgs& ka, int rows, CUtensorMap* k, CUtensorMap* v);
+// Floats of scratch for ka.few_rows (16 or 32).
+size_t chunk_few_floats(const ChunkArgs& ka);
+// Every request of ka.few_rows rows (token, head of the group) or less.
+int launch_chunk_few(ChunkArgs& ka, float* scratch, cudaStream_t stream);
+
+}  // namespace subspec
