@@ -318,6 +318,28 @@ def check(rc: int, what: str) -> None:
     raise SubspecError(f"{what}: {msg}")
 
 
+def on_device(fn, args, device, what: str) -> None:
+    """Call an entry point on `device`'s current stream, with `device` current for its launches."""
+    import torch
+
+    index = device.index
+    if index == torch.cuda.current_device():
+        check(fn(C.byref(args), _raw_stream(index)), what)
+    else:
+        with torch.cuda.device(index):
+            check(fn(C.byref(args), _raw_stream(index)), what)
+
+
+def _raw_stream(index: int) -> int:
+    import torch
+
+    global _raw_stream
+    # torch.cuda.current_stream builds a Stream object (2 us of a small call's 15); torch's own compilers read the handle
+    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    _raw_stream = get or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return _raw_stream(index)
+
+
 def dev_status_text(word: int) -> str:
     return "; ".join(t for bit, t in _DEV_TEXT.items() if word & bit)
 

@@ -11,6 +11,7 @@ package leave them: `KvCachePool.cache_data`, `DevicePagePool.page_table` / `kv_
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import Optional
 
@@ -199,19 +200,20 @@ def tree_attention_static(q: torch.Tensor, key_cache: torch.Tensor, value_cache:
 
 
 def _aligned(t: torch.Tensor) -> bool:
-    """Whether every row of the last axis can be read 16 bytes at a time."""
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in t.stride()[:-1])
+    """Whether the rows of a [tokens, heads, head_dim] tensor can be read 16 bytes at a time."""
+    s0, s1, s2 = t.stride()
+    return s2 == 1 and not (s0 | s1) & 7 and not t.data_ptr() & 15
 
 
-def _check_pool(pool: torch.Tensor, layer: int) -> None:
-    if pool.dim() != 6 or pool.shape[2] != 2 or not pool.is_contiguous() or \
-            pool.dtype not in (torch.bfloat16, torch.float16):
+def _check_pool(pool: torch.Tensor, layer: int):
+    shape = pool.shape
+    if len(shape) != 6 or shape[2] != 2 or not pool.is_contiguous() or pool.dtype not in (torch.bfloat16, torch.float16):
         raise ValueError("pool must be a contiguous bf16 or fp16 [layers, pages, 2, page_len, kv_heads, head_dim] tensor")
-    if not 0 <= int(layer) < pool.shape[0]:
+    if not 0 <= layer < shape[0]:
         raise ValueError("layer outside the pool")
+    return shape
 
 
-@torch.no_grad()
 def append_paged_kv_slots(pool: torch.Tensor, layer: int, k: torch.Tensor, v: torch.Tensor, *, slot_map: torch.Tensor,
                           status: Optional[torch.Tensor] = None) -> None:
     """k, v [tokens, kv_heads, head_dim] of packed requests -> rows `slot_map[t]` of layer `layer`.
@@ -219,86 +221,80 @@ def append_paged_kv_slots(pool: torch.Tensor, layer: int, k: torch.Tensor, v: to
     `slot_map` int64 [>= tokens] as `DevicePagePool.plan_chunks` leaves it: page * page_len + row, all different;
     negative ones are skipped (a padded batch), one past the pool sets `status`.  k and v may be slices of a fused
     projection."""
-    _check_pool(pool, layer)
-    L, P, _, page_len, H, D = (int(x) for x in pool.shape)
-    if k.dim() != 3 or k.shape != v.shape or tuple(k.shape[1:]) != (H, D) or k.dtype != pool.dtype or \
-            v.dtype != pool.dtype or k.device != pool.device or v.device != pool.device:
+    L, P, _, page_len, H, D = _check_pool(pool, layer)
+    shape, dev = k.shape, pool.device
+    if len(shape) != 3 or shape != v.shape or shape[1] != H or shape[2] != D or k.dtype != pool.dtype or \
+            v.dtype != pool.dtype or k.device != dev or v.device != dev:
         raise ValueError("k and v must be [tokens, kv_heads, head_dim] tensors of the pool's type on its device")
-    T = int(k.shape[0])
-    if slot_map.dtype != torch.int64 or slot_map.device != pool.device or slot_map.dim() != 1 or \
-            slot_map.numel() < T or not slot_map.is_contiguous():
+    T = shape[0]
+    if slot_map.dtype != torch.int64 or slot_map.device != dev or slot_map.dim() != 1 or slot_map.shape[0] < T or \
+            not slot_map.is_contiguous():
         raise ValueError("slot_map must be a contiguous int64 tensor on the pool's device with an entry per token")
     if D % 8:
         raise ValueError("head_dim must be a multiple of 8")
     if T == 0:
         return
-    k, v = (x if _aligned(x) else x.clone(memory_format=torch.contiguous_format) for x in (k, v))
-    a = _lib.KvAppendSlotsArgs()
-    a.struct_size = C.sizeof(_lib.KvAppendSlotsArgs)
-    a.tokens, a.num_kv_heads, a.head_dim = T, H, D
-    a.layer, a.layers, a.num_pages, a.page_len = int(layer), L, P, page_len
-    a.pool, a.k, a.v, a.slot_map = pool.data_ptr(), k.data_ptr(), v.data_ptr(), slot_map.data_ptr()
-    a.k_token_stride, a.k_head_stride = int(k.stride(0)), int(k.stride(1))
-    a.v_token_stride, a.v_head_stride = int(v.stride(0)), int(v.stride(1))
-    a.dev_status = 0 if status is None else status.data_ptr()
-    with torch.cuda.device(pool.device):
-        stream = torch.cuda.current_stream(pool.device).cuda_stream
-        _lib.check(_lib.lib().subspec_kv_append_slots(C.byref(a), C.c_void_p(stream)), "subspec_kv_append_slots")
+    if not _aligned(k):
+        k = k.detach().clone(memory_format=torch.contiguous_format)
+    if not _aligned(v):
+        v = v.detach().clone(memory_format=torch.contiguous_format)
+    a = _lib.KvAppendSlotsArgs(C.sizeof(_lib.KvAppendSlotsArgs), T, H, D, layer, L, P, page_len, pool.data_ptr(),
+                               k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                               slot_map.data_ptr(), 0 if status is None else status.data_ptr())
+    _lib.on_device(_lib.lib().subspec_kv_append_slots, a, dev, "subspec_kv_append_slots")
 
 
-def _chunk_attention(what: str, q, pool, layer, page_table, kv_len, q_indptr, max_q_len, window, sinks, sm_scale, status,
-                     out, kv_splits) -> torch.Tensor:
-    _check_pool(pool, layer)
-    L, P, _, page_len, H, D = (int(x) for x in pool.shape)
-    if q.dim() != 3 or q.dtype != pool.dtype or q.device != pool.device or int(q.shape[2]) != D or D not in (64, 128):
+@functools.lru_cache(maxsize=1024)
+def _chunk_scratch_bytes(B, T, max_q_len, HQ, H, D, page_len, width, window, sinks, kv_splits) -> int:
+    """Scratch of a chunk attention call, which depends on these sizes alone."""
+    need = C.c_size_t(0)
+    a = _lib.ChunkAttnArgs(C.sizeof(_lib.ChunkAttnArgs), B, T, max_q_len, HQ, H, D, 0, 1, 1, page_len, width, _lib.BF16,
+                           window, sinks, kv_splits)
+    a.sm_scale = 1.0
+    _lib.check(_lib.lib().subspec_chunk_attention_scratch_bytes(C.byref(a), C.byref(need)), "subspec_chunk_attention_paged")
+    return need.value
+
+
+def _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, window, sinks, sm_scale, status, out,
+                     kv_splits) -> torch.Tensor:
+    L, P, _, page_len, H, D = _check_pool(pool, layer)
+    shape, dev = q.shape, pool.device
+    if len(shape) != 3 or q.dtype != pool.dtype or q.device != dev or shape[2] != D or D not in (64, 128):
         raise ValueError("q must be [tokens, q_heads, head_dim] of the pool's type and head_dim (64 or 128) on its device")
-    T, HQ = int(q.shape[0]), int(q.shape[1])
+    T, HQ, _ = shape
     if HQ < 1 or HQ % H:
         raise ValueError("q_heads must be a multiple of the pool's kv_heads")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous() or \
-            page_table.device != pool.device:
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous() or page_table.device != dev:
         raise ValueError("page_table must be a contiguous int32 [batch, pages_per_seq] tensor on the pool's device")
-    B = int(page_table.shape[0])
+    B, width = page_table.shape
     if out is None:
-        out = torch.empty(T, HQ, D, dtype=q.dtype, device=q.device)
-    elif out.dtype != q.dtype or out.shape != q.shape or out.device != q.device or not (T == 0 or _aligned(out)):
+        out = torch.empty(T, HQ, D, dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != shape or out.device != dev or not (T == 0 or _aligned(out)):
         raise ValueError("out must be a tensor of q's type and shape on q's device, its rows 16-byte aligned")
-    if max_q_len is None:
-        max_q_len = T
-    elif not 0 <= int(max_q_len):
+    max_q_len = T if max_q_len is None else int(max_q_len)
+    if max_q_len < 0:
         raise ValueError("max_q_len must not be negative")
-    a = _lib.ChunkAttnArgs()
-    a.struct_size = C.sizeof(_lib.ChunkAttnArgs)
-    a.batch, a.tokens, a.max_q_len, a.num_q_heads, a.num_kv_heads, a.head_dim = B, T, min(int(max_q_len), T), HQ, H, D
-    a.layer, a.layers, a.num_pages, a.page_len = int(layer), L, P, page_len
-    a.pages_per_seq = int(page_table.shape[1])
-    a.dtype = _lib.BF16 if q.dtype == torch.bfloat16 else _lib.F16
-    a.window, a.sinks = window, sinks
-    a.kv_splits = 0 if kv_splits is None else int(kv_splits)
-    if kv_splits is not None and not 1 <= int(kv_splits) <= 1024:
+    if kv_splits is None:
+        kv_splits = 0
+    elif not 1 <= int(kv_splits) <= 1024:
         raise ValueError("kv_splits must be between 1 and 1024")
-    a.pool, a.page_table = pool.data_ptr(), page_table.data_ptr()
-    a.kv_len, a.q_indptr = _i32(kv_len, pool.device, B, "kv_len"), _i32(q_indptr, pool.device, B + 1, "q_indptr")
+    kv_ptr, indptr_ptr = _i32(kv_len, dev, B, "kv_len"), _i32(q_indptr, dev, B + 1, "q_indptr")
     if T == 0 or B == 0:
         return out
     if not _aligned(q):
-        q = q.clone(memory_format=torch.contiguous_format)
-    a.q, a.q_token_stride, a.q_head_stride = q.data_ptr(), int(q.stride(0)), int(q.stride(1))
-    a.out, a.o_token_stride, a.o_head_stride = out.data_ptr(), int(out.stride(0)), int(out.stride(1))
-    a.sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(D)
-    a.dev_status = 0 if status is None else status.data_ptr()
-    with torch.cuda.device(pool.device):
-        need = C.c_size_t(0)
-        _lib.check(_lib.lib().subspec_chunk_attention_scratch_bytes(C.byref(a), C.byref(need)), what)
-        scratch = torch.empty(need.value, dtype=torch.uint8, device=pool.device) if need.value else None
-        if scratch is not None:
-            a.scratch, a.scratch_bytes = scratch.data_ptr(), need.value
-        stream = torch.cuda.current_stream(pool.device).cuda_stream
-        _lib.check(_lib.lib().subspec_chunk_attention_paged(C.byref(a), C.c_void_p(stream)), what)
-    return out
+        q = q.detach().clone(memory_format=torch.contiguous_format)
+    max_q_len, kv_splits = min(max_q_len, T), int(kv_splits)
+    need = _chunk_scratch_bytes(B, T, max_q_len, HQ, H, D, page_len, width, window, sinks, kv_splits)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    a = _lib.ChunkAttnArgs(C.sizeof(_lib.ChunkAttnArgs), B, T, max_q_len, HQ, H, D, layer, L, P, page_len, width,
+                           _lib.BF16 if q.dtype == torch.bfloat16 else _lib.F16, window, sinks, kv_splits,
+                           pool.data_ptr(), page_table.data_ptr(), kv_ptr, indptr_ptr, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                           1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
+                           0 if status is None else status.data_ptr(), 0 if scratch is None else scratch.data_ptr(), need)
+    _lib.on_device(_lib.lib().subspec_chunk_attention_paged, a, dev, "subspec_chunk_attention_paged")
+    return out  # (torch's allocator keeps the scratch for this stream until the kernels have passed)
 
 
-@torch.no_grad()
 def chunk_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, page_table: torch.Tensor,
                           kv_len: torch.Tensor, q_indptr: torch.Tensor, max_q_len: Optional[int] = None,
                           sm_scale: Optional[float] = None, status: Optional[torch.Tensor] = None,
@@ -312,11 +308,9 @@ def chunk_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, pa
     rows per request are chosen by it.  Rows of the output behind q_indptr[-1] are left as they were; what a token does
     not see has no influence on it, infinities and NaN included.  What `DevicePagePool.plan_chunks` returned fits as
     it is: chunk_attention_paged(q, pool, layer, page_table=plan.page_table, kv_len=plan.kv_len, q_indptr=plan.q_indptr)."""
-    return _chunk_attention("chunk_attention_paged", q, pool, layer, page_table, kv_len, q_indptr, max_q_len, 0, 0,
-                            sm_scale, status, out, kv_splits)
+    return _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, 0, 0, sm_scale, status, out, kv_splits)
 
 
-@torch.no_grad()
 def window_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, page_table: torch.Tensor,
                            kv_len: torch.Tensor, q_indptr: torch.Tensor, window: int, sinks: int = 0,
                            max_q_len: Optional[int] = None, sm_scale: Optional[float] = None,
@@ -329,5 +323,5 @@ def window_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, p
     if window < 1 or sinks < 0:
         raise ValueError("window must be at least 1 and sinks not negative")
     cap = int(page_table.shape[-1]) * int(pool.shape[3]) if page_table.dim() == 2 and pool.dim() == 6 else window
-    return _chunk_attention("window_attention_paged", q, pool, layer, page_table, kv_len, q_indptr, max_q_len,
-                            max(1, min(window, cap)), min(sinks, cap), sm_scale, status, out, kv_splits)
+    return _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, max(1, min(window, cap)),
+                            min(sinks, cap), sm_scale, status, out, kv_splits)

@@ -76,6 +76,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const int kvh = blockIdx.y, G = ka.group;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = (int)blockIdx.x % ka.splits;
+  grid_dep_launch();
 
   // ---- which request and which of its row tiles: every warp looks for itself ----
   int b = -1, qt = 0;
@@ -523,6 +524,7 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkArgs ka) {
   const subspec_chunk_attn_args& a = ka.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = ka.group;
   const long long r = (long long)blockIdx.x * 4 + warp;
+  grid_dep_wait();
   if (r >= (long long)a.tokens * a.num_q_heads) return;
   const int t = (int)(r / a.num_q_heads), head = (int)(r - (long long)t * a.num_q_heads);
   const int b = request_of(a.q_indptr, a.batch, t);
@@ -671,8 +673,7 @@ void chunk_tensor_maps(ChunkArgs& ka, int rows, CUtensorMap* k, CUtensorMap* v) 
 template <bool kHalf, int kDim>
 static int launch_chunk(ChunkArgs& ka, cudaStream_t stream) {
   const subspec_chunk_attn_args& a = ka.a;
-  const int rc = cuda_check(cudaFuncSetAttribute(chunk_attn_tc_kernel<kHalf, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)tc_smem<kDim>()));
+  const int rc = allow_smem<chunk_attn_tc_kernel<kHalf, kDim>>(tc_smem<kDim>());
   if (rc) return rc;
   CUtensorMap tmap_k, tmap_v;
   chunk_tensor_maps(ka, kTileKeys, &tmap_k, &tmap_v);
@@ -680,7 +681,8 @@ static int launch_chunk(ChunkArgs& ka, cudaStream_t stream) {
                                       tc_smem<kDim>(), stream>>>(ka, tmap_k, tmap_v);
   if (ka.splits > 1) {
     const long long rows = (long long)a.tokens * a.num_q_heads;
-    chunk_merge_kernel<kHalf, kDim><<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(ka);
+    const int rc2 = cuda_check(cudaGetLastError());
+    return rc2 ? rc2 : launch_dependent(chunk_merge_kernel<kHalf, kDim>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, ka);
   }
   return cuda_check(cudaGetLastError());
 }

@@ -97,14 +97,17 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   __shared__ int s_abort;
   const subspec_chunk_attn_args& a = ka.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = ka.group, H = a.num_kv_heads;
+  grid_dep_launch();
   if (blockIdx.x == 0 && warp == 0)
     for (int x = lane; x < a.batch; x += 32) read_request(a, x, true);
 
   // ---- the line's length, and where this CTA's run begins ----
   long long total = 0;
+  int first_tiles = 0;  // of this lane's request among the first 32
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
     const int b = b0 + lane;
     const int tiles = b < a.batch ? few_tiles(ka, read_request(a, b, false), nullptr) : 0;
+    if (b0 == 0) first_tiles = tiles;
     total += __reduce_add_sync(0xffffffffu, tiles);
   }
   total *= H;
@@ -117,7 +120,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     int b0 = 0;
     for (;; b0 += 32) {
       const int b = b0 + lane;
-      const int tiles = b < a.batch ? few_tiles(ka, read_request(a, b, false), nullptr) : 0;
+      const int tiles = b0 == 0 ? first_tiles : b < a.batch ? few_tiles(ka, read_request(a, b, false), nullptr) : 0;
       int incl = tiles;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -446,11 +449,14 @@ __global__ void __launch_bounds__(128) chunk_few_join_kernel(const ChunkArgs ka,
   const subspec_chunk_attn_args& a = ka.a;
   const int t = (int)(blockIdx.x / a.num_q_heads), head = (int)(blockIdx.x % a.num_q_heads);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = ka.group, H = a.num_kv_heads;
+  // (the lengths were there before the kernel in front began)
   const int b = request_of(a.q_indptr, a.batch, t);
-  if (b < 0) return;
-  const Request rq = read_request(a, b, false);
+  const Request rq = read_request(a, max(b, 0), false);
   const int tiles = few_tiles(ka, rq, nullptr), i = t - rq.q0;
-  if (tiles == 0 || i >= rq.n) return;
+  if (b < 0 || tiles == 0 || i >= rq.n) {
+    grid_dep_wait();
+    return;
+  }
   // tiles in front of the request, and all of them
   long long before = 0, total = 0;
   for (int x = (int)threadIdx.x; x < a.batch; x += 128) {
@@ -471,6 +477,7 @@ __global__ void __launch_bounds__(128) chunk_few_join_kernel(const ChunkArgs ka,
   const long long s0 = before + (long long)(head / G) * tiles, s1 = s0 + tiles;
   // the run that holds tile x: the largest c with floor(c total / runs) <= x
   const int c0 = (int)(((s0 + 1) * runs - 1) / total), c1 = (int)((s1 * runs - 1) / total);
+  grid_dep_wait();
   if (c0 == c1) return;  // written by the run itself
   const int grow = i * G + head % G;
   constexpr int kChunks = kDim / 8, kGroups = 128 / kChunks;
@@ -532,15 +539,15 @@ __global__ void __launch_bounds__(128) chunk_few_join_kernel(const ChunkArgs ka,
 
 template <bool kHalf, int kDim, int kMT>
 int launch(ChunkArgs& ka, cudaStream_t stream) {
-  auto kernel = chunk_attn_few_kernel<kHalf, kDim, kMT>;
-  const int rc = cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)few_smem<kDim>()));
+  const int rc = allow_smem<chunk_attn_few_kernel<kHalf, kDim, kMT>>(few_smem<kDim>());
   if (rc) return rc;
   CUtensorMap tmap_k, tmap_v;
   chunk_tensor_maps(ka, kWarpKeys, &tmap_k, &tmap_v);
-  kernel<<<kFewCtas, kFewThreads, few_smem<kDim>(), stream>>>(ka, tmap_k, tmap_v);
+  chunk_attn_few_kernel<kHalf, kDim, kMT><<<kFewCtas, kFewThreads, few_smem<kDim>(), stream>>>(ka, tmap_k, tmap_v);
+  const int launched = cuda_check(cudaGetLastError());
+  if (launched) return launched;
   const long long rows = (long long)ka.a.tokens * ka.a.num_q_heads;
-  chunk_few_join_kernel<kHalf, kDim, kMT><<<(unsigned)rows, 128, 0, stream>>>(ka, kFewCtas);
-  return cuda_check(cudaGetLastError());
+  return launch_dependent(chunk_few_join_kernel<kHalf, kDim, kMT>, dim3((unsigned)rows), dim3(128), 0, stream, ka, kFewCtas);
 }
 
 template <int kMT>

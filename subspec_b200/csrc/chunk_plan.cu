@@ -64,11 +64,28 @@ __device__ __forceinline__ int last_not_above(const int* a, int n, int x) {
   return lo;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const subspec_chunk_plan_args a) {
+// Token t's entries: request b (-1: behind the last token), its row, and the pages the request got.
+__device__ __forceinline__ void write_token(const subspec_chunk_plan_args& a, int t, int b, int pos, int pages) {
+  long long slot = -1;
+  const int pi = pos / a.page_len;
+  if (b >= 0 && pi < pages) {
+    const int pg = __ldcg(a.page_table + (size_t)b * a.pages_per_seq + pi);
+    if (pg >= 0 && pg < a.num_pages)
+      slot = (long long)pg * a.page_len + (pos - pi * a.page_len);
+    else
+      flag(a.dev_status, SUBSPEC_DEV_BAD_PAGE);
+  }
+  a.slot_map[t] = slot;
+  a.positions[t] = pos;
+  a.batch_indices[t] = b;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const subspec_chunk_plan_args a, int tokens_here) {
   extern __shared__ int sm[];
   __shared__ uint64_t s_warp[32];
   __shared__ uint64_t s_total;
   cg::cluster_group cluster = cg::this_cluster();
+  grid_dep_launch();
   const int B = a.batch, P = a.pages_per_seq, L = a.page_len;
   const int words = (a.num_pages + 31) / 32;
   const int cta = (int)blockIdx.x, ctas = (int)gridDim.x;
@@ -187,24 +204,40 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const subspec_
     }
     a.free_mask[w] = bits;
   }
+  if (!tokens_here) {  // the second kernel reads a request's kept rows from its first token's position
+    for (int b = cta * kPlanThreads + (int)threadIdx.x; b < B; b += ctas * kPlanThreads)
+      if (indptr[b] < indptr[b + 1] && indptr[b] < a.max_tokens) a.positions[indptr[b]] = base[b];
+    return;
+  }
   for (int t = cta * kPlanThreads + (int)threadIdx.x; t < a.max_tokens; t += ctas * kPlanThreads) {
-    int b = -1, pos = 0;
-    long long slot = -1;
-    if (t < tokens) {
-      b = last_not_above(indptr, B, t);
-      pos = base[b] + t - indptr[b];
-      const int pi = pos / L;
-      if (pi < P && pi < keep[b] + min(max(given - first[b], 0), first[b + 1] - first[b])) {
-        const int pg = __ldcg(a.page_table + (size_t)b * P + pi);
-        if (pg >= 0 && pg < a.num_pages)
-          slot = (long long)pg * L + (pos - pi * L);
-        else
-          flag(a.dev_status, SUBSPEC_DEV_BAD_PAGE);
-      }
+    const int b = t < tokens ? last_not_above(indptr, B, t) : -1;
+    write_token(a, t, b, b < 0 ? 0 : base[b] + t - indptr[b],
+                b < 0 ? 0 : keep[b] + min(max(given - first[b], 0), first[b + 1] - first[b]));
+  }
+}
+
+// The tokens of a large step, on all SMs.
+constexpr int kTokenThreads = 512;
+__global__ void __launch_bounds__(kTokenThreads) chunk_plan_tokens_kernel(const subspec_chunk_plan_args a) {
+  extern __shared__ int sm[];
+  const int B = a.batch;
+  int* indptr = sm;            // [B + 1]
+  int* base = indptr + B + 1;  // [B]
+  int* pages = base + B;       // [B]
+  grid_dep_wait();
+  for (int b = (int)threadIdx.x; b <= B; b += kTokenThreads) {
+    const int at = a.q_indptr[b];
+    indptr[b] = at;
+    if (b < B) {
+      base[b] = at < a.max_tokens ? __ldcg(a.positions + at) : 0;  // (a request without tokens reads another's: not used)
+      pages[b] = a.n_pages[b];
     }
-    a.slot_map[t] = slot;
-    a.positions[t] = pos;
-    a.batch_indices[t] = b;
+  }
+  __syncthreads();
+  const int tokens = indptr[B];
+  for (int t = (int)(blockIdx.x * kTokenThreads + threadIdx.x); t < a.max_tokens; t += (int)(gridDim.x * kTokenThreads)) {
+    const int b = t < tokens ? last_not_above(indptr, B, t) : -1;
+    write_token(a, t, b, b < 0 ? 0 : base[b] + t - indptr[b], b < 0 ? 0 : pages[b]);
   }
 }
 
@@ -251,14 +284,15 @@ extern "C" int subspec_chunk_plan(const subspec_chunk_plan_args* args, subspec_s
   const size_t words = ((size_t)a.num_pages + 31) / 32;
   const size_t smem = sizeof(int) * (4 * (size_t)a.batch + 2 + words);
   if (smem > 200 * 1024) return SUBSPEC_EUNSUPPORTED;
-  if (smem > 48 * 1024) {
-    const int rc =
-        cuda_check(cudaFuncSetAttribute(chunk_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    if (rc) return rc;
-  }
-  // a CTA for every 1024 tokens or requests' page lists, at most one cluster of eight
-  long long ctas = (a.max_tokens + kPlanThreads - 1) / kPlanThreads;
+  int rc = allow_smem<chunk_plan_kernel>(200 * 1024);
+  if (!rc) rc = allow_smem<chunk_plan_tokens_kernel>(200 * 1024);
+  if (rc) return rc;
+  // Up to 8192 tokens the planning CTAs write them too; more go to a kernel of their own on all SMs.
+  const int tokens_here = a.max_tokens <= kPlanMaxCtas * kPlanThreads;
+  // a CTA for every 1024 tokens, page lists of 32 requests or 32768 pages, at most one cluster of eight
+  long long ctas = tokens_here ? (a.max_tokens + kPlanThreads - 1) / kPlanThreads : 1;
   if ((a.batch + 31) / 32 > ctas) ctas = (a.batch + 31) / 32;
+  if (words / 1024 > (size_t)ctas) ctas = words / 1024;
   int n = 1;
   while (n < kPlanMaxCtas && n < ctas) n *= 2;
   cudaLaunchConfig_t cfg = {};
@@ -272,7 +306,11 @@ extern "C" int subspec_chunk_plan(const subspec_chunk_plan_args* args, subspec_s
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_check(cudaLaunchKernelEx(&cfg, chunk_plan_kernel, a));
+  rc = cuda_check(cudaLaunchKernelEx(&cfg, chunk_plan_kernel, a, tokens_here));
+  if (rc || tokens_here) return rc;
+  const long long blocks = ((long long)a.max_tokens + kTokenThreads - 1) / kTokenThreads;
+  return launch_dependent(chunk_plan_tokens_kernel, dim3((unsigned)(blocks < 2 * kNumSMs ? blocks : 2 * kNumSMs)), dim3(kTokenThreads),
+                          sizeof(int) * (3 * (size_t)a.batch + 1), cfg.stream, a);
 }
 
 extern "C" int subspec_kv_append_slots(const subspec_kv_append_slots_args* args, subspec_stream_t stream) {

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/subspec_b200.h"
 
 namespace subspec {
@@ -18,7 +20,42 @@ constexpr int kNumSMs = 148;  // B200: 2 dies x 74 SMs
 int cuda_fail(cudaError_t e);
 inline int cuda_check(cudaError_t e) { return e == cudaSuccess ? SUBSPEC_OK : cuda_fail(e); }
 
+// Dynamic shared memory above 48 KB for a kernel: asked for once per device (and per kernel: a template parameter).
+template <auto kKernel>
+int allow_smem(size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  const int rc = cuda_check(cudaGetDevice(&dev));
+  if (rc) return rc;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return SUBSPEC_OK;
+  const int set = cuda_check(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  if (set == SUBSPEC_OK) done.fetch_or(bit, std::memory_order_relaxed);
+  return set;
+}
+
 #ifdef __CUDACC__
+
+// Launch as a programmatic dependent of the kernel in front: its blocks may start, up to grid_dep_wait, once all of that
+// one's have called grid_dep_launch or ended.
+template <typename... Params, typename... Args>
+int launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+__device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Everything the kernel in front wrote is visible from here on.  Every block calls it, those with nothing to do too: a
+// grid that ended before the one in front would let the kernel behind it start early.
+__device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ float ex2f(float x) {
   float y;

@@ -98,7 +98,15 @@ class DevicePagePool:
                                     kv_page_indices=self.kv_page_indices, kv_last_page_len=self.kv_last_page_len,
                                     batch_indices=self.batch_indices, positions=self.positions)
 
-    @torch.no_grad()
+    def _lengths(self, t: torch.Tensor, name: str) -> torch.Tensor:
+        if t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
+            if t.is_floating_point():
+                raise ValueError(f"{name} must hold one whole number per request")
+            t = t.to(self.device, torch.int32).contiguous()
+        if t.numel() != self.batch:
+            raise ValueError(f"{name} must hold one whole number per request")
+        return t
+
     def plan_chunks(self, n_new: torch.Tensor, *, set_len: Optional[torch.Tensor] = None) -> ChunkPlan:
         """Block tables and slot maps of a step in which request b brings `n_new[b]` tokens (0 allowed), on the current
         stream (no synchronisation): `getKvCacheBatchPosition` for chunks of any lengths.
@@ -110,27 +118,18 @@ class DevicePagePool:
         tokens of a step.  Running out of pages or of `max_append` is reported by `check_status`."""
         if self.max_append < 1:
             raise ValueError("plan_chunks needs a pool made with max_append: the most tokens a step brings")
-        a = _lib.ChunkPlanArgs()
-        a.struct_size = C.sizeof(_lib.ChunkPlanArgs)
-        a.batch, a.num_pages, a.page_len, a.pages_per_seq = self.batch, self.num_pages, self.page_len, self.pages_per_seq
-        a.max_tokens = self.max_append
-        keep = []
-        for name, t in (("n_new", n_new), ("set_len", set_len)):
-            if t is None:
-                continue
-            if t.is_floating_point() or t.numel() != self.batch:
-                raise ValueError(f"{name} must hold one whole number per request")
-            t = t.to(self.device, torch.int32).contiguous()
-            keep.append(t)
-            setattr(a, name, t.data_ptr())
-        a.free_mask, a.page_table, a.n_pages = self.free_mask.data_ptr(), self.page_table.data_ptr(), self.n_pages.data_ptr()
-        a.kv_len, a.kv_last_page_len = self.kv_len.data_ptr(), self.kv_last_page_len.data_ptr()
-        a.q_indptr, a.slot_map = self.seq_indptr.data_ptr(), self.slot_map.data_ptr()
-        a.positions, a.batch_indices = self.positions.data_ptr(), self.batch_indices.data_ptr()
-        a.dev_status = self.status.data_ptr()
-        with torch.cuda.device(self.device):
-            stream = torch.cuda.current_stream(self.device).cuda_stream
-            _lib.check(_lib.lib().subspec_chunk_plan(C.byref(a), C.c_void_p(stream)), "subspec_chunk_plan")
+        if set_len is None:
+            set_ptr = 0
+        else:
+            set_len = self._lengths(set_len, "set_len")
+            set_ptr = set_len.data_ptr()
+        n_new = self._lengths(n_new, "n_new")
+        a = _lib.ChunkPlanArgs(
+            C.sizeof(_lib.ChunkPlanArgs), self.batch, self.num_pages, self.page_len, self.pages_per_seq, self.max_append,
+            self.free_mask.data_ptr(), self.page_table.data_ptr(), self.n_pages.data_ptr(), self.kv_len.data_ptr(),
+            self.kv_last_page_len.data_ptr(), set_ptr, n_new.data_ptr(), self.seq_indptr.data_ptr(),
+            self.slot_map.data_ptr(), self.positions.data_ptr(), self.batch_indices.data_ptr(), self.status.data_ptr())
+        _lib.on_device(_lib.lib().subspec_chunk_plan, a, self.device, "subspec_chunk_plan")
         return ChunkPlan(q_indptr=self.seq_indptr, slot_map=self.slot_map, positions=self.positions,
                          batch_indices=self.batch_indices, page_table=self.page_table, kv_len=self.kv_len)
 
