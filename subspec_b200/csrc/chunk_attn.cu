@@ -28,9 +28,10 @@ namespace {
 //               128 scores, m = the running maximum, and writes P = 2^(S c - m) as 16-bit pairs over the first half of
 //               the columns it read, summing P in fp32.  m moves, and the row of O in tensor memory is rescaled, only
 //               when the maximum has run 2^8 ahead of it.
-//   warps 8, 9  one MMA issuer per block: S = Q K^T (128 x 128 x head_dim, both K-major in shared memory), O += P V (P
-//               from tensor memory, V MN-major as the cache has it).  S of the next tile goes over P as soon as O += P V
-//               is issued: the MMAs of a thread run in order.  While one block is in its softmax the other's MMAs run.
+//   warp 8      issues the MMAs, one block after the other: O += P V (P from tensor memory, V MN-major as the cache has
+//               it), in two halves of 64 cache rows as their P comes, then S = Q K^T of the next tile (128 x 128 x
+//               head_dim, both K-major in shared memory) over the P just consumed: the MMAs of a thread run in order.
+//               While one block is in its softmax the other's MMAs run.  (Warp 9 idles.)
 //   warp 10     brings the K tiles, warp 11 the V tiles, into a ring of five entries, K(0), V(0), K(1), V(1), ...
 //
 // A tile lies in shared memory as 16 groups of 8 rows; a group as one (head_dim 64) or two halves of 64 dims, a half as
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     chunk_attn_tc_kernel(const ChunkArgs ka, const __grid_constant__ CUtensorMap tmap_k,
                          const __grid_constant__ CUtensorMap tmap_v) {
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t full[kRing], empty[kRing], s_ready[2], p_ready[2], o_done[2], q_ready, fix;
+  __shared__ __align__(8) uint64_t full[kRing], empty[kRing], s_ready[2], p_ready[2][2], o_done[2], q_ready, fix, drained;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   constexpr int kHalves = kDim / 64;
@@ -157,15 +158,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kRing; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], (uint32_t)nblk);
+      mbar_init(&empty[s], 1);
     }
     for (int k = 0; k < 2; ++k) {
       mbar_init(&s_ready[k], 1);
-      mbar_init(&p_ready[k], 4);
+      mbar_init(&p_ready[k][0], 4);
+      mbar_init(&p_ready[k][1], 4);
       mbar_init(&o_done[k], 1);
     }
     mbar_init(&q_ready, kCtaRows);
     mbar_init(&fix, 1);
+    mbar_init(&drained, 1);
     mbar_init_fence();
     s_abort = 0;
   }
@@ -281,6 +284,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               pk[j] = pack16<kHalf>(p0, p1);
             }
             tmem_st16(lane_base + 16 * c, pk);
+            if (c & 1) {  // half of the tile: its share of O += P V can begin
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_ready[blk][c >> 1]);
+            }
           }
         };
         if (masked)
@@ -291,10 +300,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         f2_unpack(sm2[0], e0, e1);
         f2_unpack(sm2[1], e2, e3);
         l = l * alpha + ((e0 + e1) + (e2 + e3));
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[blk]);
         ++done;
       }
       // ---- the result: O / l ----
@@ -362,60 +367,103 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp < kLoadWarp) {
-      // ================= MMA issue, one warp per block, an elected lane issues =================
-      const int blk = warp - kIssuerWarp;
-      if (blk < nblk) {
+      // ================= MMA issue: one warp for both blocks, an elected lane issues =================
+      // One issuer, one block after the other: with an issuer per block the two blocks' MMAs interleave, both get
+      // their scores at the same time and then both sit in their softmax while the tensor cores idle (4660 cycles a
+      // tile against 2048 of MMAs).
+      if (warp == kIssuerWarp) {
         constexpr uint32_t idesc_s = tc_idesc(kBlockRows, kTileKeys, false, kHalf);
         constexpr uint32_t idesc_o = tc_idesc(kBlockRows, kDim, true, kHalf);
-        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + (uint32_t)blk * kBlockCols;
-        const uint32_t q_u32 = smem_u32(qtiles) + (uint32_t)blk * kQBlockBytes, ring_u32 = smem_u32(ring);
-        int bfirst, blast;
-        block_pos(blk, bfirst, blast);
-        int last_seen = -1;
-        for (int i = ntiles - 1; i >= 0 && last_seen < 0; --i)
-          if (block_sees(bfirst, blast, tiles.first_row(i0 + i))) last_seen = i;
-        int e = 0;         // ring entry
-        uint32_t ph = 0;   // and its phase
-        uint32_t done = 0;
-        bool ok = __all_sync(0xffffffffu, tc_wait(&q_ready, 0, abort_flag));
-        bool issued = false;
-        for (int x = 0; x < 2 * ntiles && ok; ++x) {
-          // entries in the order they come: K(0), V(0), K(1), ...
-          const int i = x >> 1;
-          const bool sees = block_sees(bfirst, blast, tiles.first_row(i0 + i));
-          ok = __all_sync(0xffffffffu, tc_wait(&full[e], ph, abort_flag));
-          if (ok && sees && (x & 1)) ok = __all_sync(0xffffffffu, tc_wait(&p_ready[blk], done & 1u, abort_flag));
-          if (!ok) break;
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint32_t q_u32 = smem_u32(qtiles), ring_u32 = smem_u32(ring);
+        int bfirst[2], blast[2], last_seen[2] = {-1, -1};
+        uint32_t done[2] = {0, 0};
+        block_pos(0, bfirst[0], blast[0]);
+        block_pos(nblk - 1, bfirst[1], blast[1]);
+        auto sees = [&](int blk, int i) { return blk < nblk && block_sees(bfirst[blk], blast[blk], tiles.first_row(i0 + i)); };
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk)
+          for (int i = ntiles - 1; i >= 0 && last_seen[blk] < 0; --i)
+            if (sees(blk, i)) last_seen[blk] = i;
+        auto issue_s = [&](int blk, uint32_t tile) {
+#pragma unroll
+          for (int ks = 0; ks < kDim / 16; ++ks)
+            tc_mma_f16_ss(tm + (uint32_t)blk * kBlockCols,
+                          tc_desc(q_u32 + (uint32_t)(blk * kQBlockBytes + (ks >> 2) * kQHalfBytes + (ks & 3) * 32), 16),
+                          tc_desc(tile + (uint32_t)((ks >> 2) * 1024 + (ks & 3) * 32), 16, kGroupBytes), idesc_s, ks > 0 ? 1u : 0u);
+          tc_commit(&s_ready[blk]);
+        };
+        auto issue_o = [&](int blk, int half, uint32_t tile) {
+#pragma unroll
+          for (int x = 0; x < kTileKeys / 32; ++x) {
+            const int ks = half * (kTileKeys / 32) + x;
+            tc_mma_f16_ta(tm + (uint32_t)blk * kBlockCols + kOCol, tm + (uint32_t)blk * kBlockCols + (uint32_t)(8 * ks),
+                          tc_desc(tile + (uint32_t)(ks * 2 * kGroupBytes), 1024, kGroupBytes), idesc_o, (done[blk] > 0 || ks > 0) ? 1u : 0u);
+          }
+        };
+        auto wait = [&](uint64_t* bar, uint32_t parity) {
+          const bool ok = __all_sync(0xffffffffu, tc_wait(bar, parity, abort_flag));
           tc_fence_after();
-          const uint32_t tile = ring_u32 + (uint32_t)(e * kTileBytes);
+          return ok;
+        };
+        int e = 0;        // ring entry, in the order they come: K(0), V(0), K(1), ...
+        uint32_t ph = 0;  // and its phase
+        auto next = [&]() {
+          if (++e == kRing) e = 0, ph ^= 1u;
+        };
+        bool issued = false;
+        bool ok = wait(&q_ready, 0) && wait(&full[0], 0);
+        if (ok) {
           if (elect_one()) {
-            if (!sees) {
-              mbar_arrive(&empty[e]);
-            } else if (!(x & 1)) {
 #pragma unroll
-              for (int ks = 0; ks < kDim / 16; ++ks)
-                tc_mma_f16_ss(tm, tc_desc(q_u32 + (uint32_t)((ks >> 2) * kQHalfBytes + (ks & 3) * 32), 16),
-                              tc_desc(tile + (uint32_t)((ks >> 2) * 1024 + (ks & 3) * 32), 16, kGroupBytes), idesc_s, ks > 0 ? 1u : 0u);
-              tc_commit(&s_ready[blk]);
-              tc_commit(&empty[e]);
-            } else {
-#pragma unroll
-              for (int ks = 0; ks < kTileKeys / 16; ++ks)
-                tc_mma_f16_ta(tm + kOCol, tm + (uint32_t)(8 * ks), tc_desc(tile + (uint32_t)(ks * 2 * kGroupBytes), 1024, kGroupBytes),
-                              idesc_o, (done > 0 || ks > 0) ? 1u : 0u);
-              tc_commit(&empty[e]);
-              if (i == last_seen) tc_commit(&o_done[blk]);
-            }
+            for (int blk = 0; blk < 2; ++blk)
+              if (sees(blk, 0)) issue_s(blk, ring_u32);
+            tc_commit(&empty[0]);
           }
           __syncwarp();
-          issued = issued || sees;
-          if (sees && (x & 1)) ++done;
-          if (++e == kRing) e = 0, ph ^= 1u;
+          issued = true;
+          next();
+        }
+        for (int i = 0; i < ntiles && ok; ++i) {
+          const int ve = e;
+          ok = wait(&full[ve], ph);
+          next();
+          const int ke = e;
+          if (ok && i + 1 < ntiles) ok = wait(&full[ke], ph);
+          if (!ok) break;
+          const uint32_t v_tile = ring_u32 + (uint32_t)(ve * kTileBytes), k_tile = ring_u32 + (uint32_t)(ke * kTileBytes);
+#pragma unroll
+          for (int blk = 0; blk < 2; ++blk) {
+            if (sees(blk, i)) {
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                if (!ok || !(ok = wait(&p_ready[blk][half], done[blk] & 1u))) break;
+                if (elect_one()) {
+                  issue_o(blk, half, v_tile);
+                  if (half == 1 && i == last_seen[blk]) tc_commit(&o_done[blk]);
+                }
+                __syncwarp();
+              }
+              if (!ok) break;
+              ++done[blk];
+            }
+            if (i + 1 < ntiles && sees(blk, i + 1)) {  // over the P just consumed: the MMAs of a thread run in order
+              if (elect_one()) issue_s(blk, k_tile);
+              __syncwarp();
+            }
+          }
+          if (!ok) break;
+          if (elect_one()) {
+            tc_commit(&empty[ve]);
+            if (i + 1 < ntiles) tc_commit(&empty[ke]);
+          }
+          __syncwarp();
+          if (i + 1 < ntiles) next();
         }
         if (!ok && issued) {  // gave up: let the MMAs in flight finish before tensor memory is freed
-          if (elect_one()) tc_commit(&o_done[blk]);
+          if (elect_one()) tc_commit(&drained);
           __syncwarp();
-          mbar_wait_bounded(&o_done[blk], 0);
+          mbar_wait_bounded(&drained, 0);
         }
       }
     } else {
