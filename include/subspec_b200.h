@@ -908,9 +908,8 @@ SUBSPEC_API int subspec_kv_append_slots(const subspec_kv_append_slots_args* args
  * q / out [tokens, num_q_heads, head_dim] in the pool's type with element strides; query head h reads KV head
  * h / (num_q_heads / num_kv_heads); head_dim 64 or 128.  Softmax in fp32.  max_q_len: no request of the call brings
  * more tokens (a request that does sets SUBSPEC_DEV_BAD_COUNT and its last tokens get no output).
- * kv_splits: cache ranges for several CTAs per query tile, 0 = chosen from the sizes.  scratch:
- * subspec_chunk_attention_scratch_bytes of the same arguments, 16-byte aligned, owned by the call until the stream has
- * passed it; need not be initialised. */
+ * scratch: subspec_chunk_attention_scratch_bytes of the same arguments, 16-byte aligned, owned by the call until the
+ * stream has passed it; need not be initialised. */
 typedef struct subspec_chunk_attn_args {
   uint32_t struct_size;
   int32_t batch;
@@ -927,7 +926,7 @@ typedef struct subspec_chunk_attn_args {
   int32_t dtype;     /* SUBSPEC_BF16 or SUBSPEC_F16: pool, q and out alike */
   int32_t window;    /* 0: none */
   int32_t sinks;
-  int32_t kv_splits;
+  int32_t reserved;
   const void* pool;
   const int32_t* page_table; /* [batch, pages_per_seq] */
   const int32_t* kv_len;     /* [batch] */

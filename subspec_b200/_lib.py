@@ -228,7 +228,7 @@ class ChunkAttnArgs(C.Structure):
         ("struct_size", _u32), ("batch", _i32), ("tokens", _i32), ("max_q_len", _i32), ("num_q_heads", _i32),
         ("num_kv_heads", _i32), ("head_dim", _i32), ("layer", _i32), ("layers", _i32), ("num_pages", _i32),
         ("page_len", _i32), ("pages_per_seq", _i32), ("dtype", _i32), ("window", _i32), ("sinks", _i32),
-        ("kv_splits", _i32), ("pool", _vp), ("page_table", _vp), ("kv_len", _vp), ("q_indptr", _vp), ("q", _vp),
+        ("reserved", _i32), ("pool", _vp), ("page_table", _vp), ("kv_len", _vp), ("q_indptr", _vp), ("q", _vp),
         ("q_token_stride", _i64), ("q_head_stride", _i64), ("out", _vp), ("o_token_stride", _i64),
         ("o_head_stride", _i64), ("sm_scale", _f64), ("dev_status", _vp), ("scratch", _vp),
         ("scratch_bytes", C.c_size_t),

@@ -245,18 +245,18 @@ def append_paged_kv_slots(pool: torch.Tensor, layer: int, k: torch.Tensor, v: to
 
 
 @functools.lru_cache(maxsize=1024)
-def _chunk_scratch_bytes(B, T, max_q_len, HQ, H, D, page_len, width, window, sinks, kv_splits) -> int:
+def _chunk_scratch_bytes(B, T, max_q_len, HQ, H, D, page_len, width, window, sinks) -> int:
     """Scratch of a chunk attention call, which depends on these sizes alone."""
     need = C.c_size_t(0)
     a = _lib.ChunkAttnArgs(C.sizeof(_lib.ChunkAttnArgs), B, T, max_q_len, HQ, H, D, 0, 1, 1, page_len, width, _lib.BF16,
-                           window, sinks, kv_splits)
+                           window, sinks)
     a.sm_scale = 1.0
     _lib.check(_lib.lib().subspec_chunk_attention_scratch_bytes(C.byref(a), C.byref(need)), "subspec_chunk_attention_paged")
     return need.value
 
 
-def _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, window, sinks, sm_scale, status, out,
-                     kv_splits) -> torch.Tensor:
+def _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, window, sinks, sm_scale, status,
+                     out) -> torch.Tensor:
     L, P, _, page_len, H, D = _check_pool(pool, layer)
     shape, dev = q.shape, pool.device
     if len(shape) != 3 or q.dtype != pool.dtype or q.device != dev or shape[2] != D or D not in (64, 128):
@@ -274,20 +274,16 @@ def _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, wi
     max_q_len = T if max_q_len is None else int(max_q_len)
     if max_q_len < 0:
         raise ValueError("max_q_len must not be negative")
-    if kv_splits is None:
-        kv_splits = 0
-    elif not 1 <= int(kv_splits) <= 1024:
-        raise ValueError("kv_splits must be between 1 and 1024")
     kv_ptr, indptr_ptr = _i32(kv_len, dev, B, "kv_len"), _i32(q_indptr, dev, B + 1, "q_indptr")
     if T == 0 or B == 0:
         return out
     if not _aligned(q):
         q = q.detach().clone(memory_format=torch.contiguous_format)
-    max_q_len, kv_splits = min(max_q_len, T), int(kv_splits)
-    need = _chunk_scratch_bytes(B, T, max_q_len, HQ, H, D, page_len, width, window, sinks, kv_splits)
+    max_q_len = min(max_q_len, T)
+    need = _chunk_scratch_bytes(B, T, max_q_len, HQ, H, D, page_len, width, window, sinks)
     scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     a = _lib.ChunkAttnArgs(C.sizeof(_lib.ChunkAttnArgs), B, T, max_q_len, HQ, H, D, layer, L, P, page_len, width,
-                           _lib.BF16 if q.dtype == torch.bfloat16 else _lib.F16, window, sinks, kv_splits,
+                           _lib.BF16 if q.dtype == torch.bfloat16 else _lib.F16, window, sinks, 0,
                            pool.data_ptr(), page_table.data_ptr(), kv_ptr, indptr_ptr, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
                            1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
                            0 if status is None else status.data_ptr(), 0 if scratch is None else scratch.data_ptr(), need)
@@ -298,7 +294,7 @@ def _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, wi
 def chunk_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, page_table: torch.Tensor,
                           kv_len: torch.Tensor, q_indptr: torch.Tensor, max_q_len: Optional[int] = None,
                           sm_scale: Optional[float] = None, status: Optional[torch.Tensor] = None,
-                          out: Optional[torch.Tensor] = None, kv_splits: Optional[int] = None) -> torch.Tensor:
+                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of packed chunks over the paged cache: q [tokens, q_heads, head_dim (64 or 128)] -> the same
     shape (into `out` when given: a captured graph needs a buffer that outlives the capture).
 
@@ -308,7 +304,7 @@ def chunk_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, pa
     rows per request are chosen by it.  Rows of the output behind q_indptr[-1] are left as they were; what a token does
     not see has no influence on it, infinities and NaN included.  What `DevicePagePool.plan_chunks` returned fits as
     it is: chunk_attention_paged(q, pool, layer, page_table=plan.page_table, kv_len=plan.kv_len, q_indptr=plan.q_indptr)."""
-    return _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, 0, 0, sm_scale, status, out, kv_splits)
+    return _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, 0, 0, sm_scale, status, out)
 
 
 def window_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, page_table: torch.Tensor,
@@ -324,4 +320,4 @@ def window_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, p
         raise ValueError("window must be at least 1 and sinks not negative")
     cap = int(page_table.shape[-1]) * int(pool.shape[3]) if page_table.dim() == 2 and pool.dim() == 6 else window
     return _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, max(1, min(window, cap)),
-                            min(sinks, cap), sm_scale, status, out, kv_splits)
+                            min(sinks, cap), sm_scale, status, out)

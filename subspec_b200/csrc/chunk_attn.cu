@@ -20,18 +20,26 @@ namespace {
 // ------------------------------------------------------------------------------------------------------------------
 // Tiles on the tensor cores.
 //
+// The work of the call is one line of row tiles -- requests, their KV heads, their tiles of 256 rows one behind the
+// other, each as long as it has cache tiles (and one more for its start and end) -- cut into equal runs, one per CTA, one
+// CTA an SM: 224 row tiles are otherwise two rounds of 148 SMs, the second half empty, and a lone short chunk behind a
+// long cache keeps four.  A row tile that a cut falls into leaves unnormalised parts in scratch, which a second kernel
+// joins; short row tiles are not cut.
+//
 // The rows of the problem are (token, head of the GQA group) pairs, token-major, so that a block of 128 rows is a run
 // of neighbouring tokens: their KV head's cache rows are read once for the whole group, and the causal border crosses
-// few tiles.  One CTA = 256 rows of one (request, KV head), two blocks that share every K / V tile of 128 cache rows:
+// few tiles.  A row tile = 256 rows of one (request, KV head), two blocks that share every K / V tile of 128 cache rows:
 //
 //   warps 0-7   softmax, four warps per block: thread = query row = lane of tensor memory.  Per tile a thread reads its
-//               128 scores, m = the running maximum, and writes P = 2^(S c - m) as 16-bit pairs over the first half of
-//               the columns it read, summing P in fp32.  m moves, and the row of O in tensor memory is rescaled, only
-//               when the maximum has run 2^8 ahead of it.
+//               128 scores and writes P = 2^(S c - m) as 16-bit pairs over the first half of the columns it read,
+//               summing P in fp32.  m, the reference point, is the maximum of the first tile, and moves (the row of O in
+//               tensor memory is rescaled) only when the sums say that a later score has run far ahead of it.  They also
+//               bring the row's Q.
 //   warp 8      issues the MMAs, one block after the other: O += P V (P from tensor memory, V MN-major as the cache has
 //               it), in two halves of 64 cache rows as their P comes, then S = Q K^T of the next tile (128 x 128 x
 //               head_dim, both K-major in shared memory) over the P just consumed: the MMAs of a thread run in order.
-//               While one block is in its softmax the other's MMAs run.  (Warp 9 idles.)
+//               While one block is in its softmax the other's MMAs run.
+//   warp 9      walks the run and hands out its pieces.
 //   warp 10     brings the K tiles, warp 11 the V tiles, into a ring of five entries, K(0), V(0), K(1), V(1), ...
 //
 // A tile lies in shared memory as 16 groups of 8 rows; a group as one (head_dim 64) or two halves of 64 dims, a half as
@@ -45,27 +53,207 @@ constexpr int kBlockRows = 128;
 constexpr int kCtaRows = 2 * kBlockRows;
 constexpr int kRing = 5;
 constexpr int kChunkThreads = 384;
-constexpr int kIssuerWarp = 8, kLoadWarp = 10;
+constexpr int kIssuerWarp = 8, kPieceWarp = 9, kLoadWarp = 10;
 constexpr uint32_t kBlockCols = 256, kOCol = 128;
-constexpr int kMinSplitTiles = 4;  // a cache range for a CTA of its own holds at least so many tiles
-
-// tiles per CTA when up to `splits` CTAs share a list of n
-__device__ __forceinline__ int per_split(int n, int splits) {
-  const int eff = max(1, min(splits, n / kMinSplitTiles));
-  return (n + eff - 1) / eff;
-}
+#ifndef KFMA
+#define KFMA 4
+#endif
+constexpr int kFmaEvery = KFMA;
+constexpr int kMinRun = 4;    // cost a run holds at least (its cache tiles and one for each row tile)
+constexpr int kSnapTiles = 8;  // row tiles of up to so many cache tiles are not cut
+constexpr int kGroups = 36;    // groups of requests whose costs are summed up side by side
 
 template <int kDim>
 constexpr size_t tc_smem() {
   return (size_t)kCtaRows * kDim * 2 + (size_t)kRing * kTileKeys * kDim * 2 + 1024;
 }
 
+// First cache row of entry i of a tile list.
+__device__ __forceinline__ int list_row(int s_tiles, int m0, int i) { return (i < s_tiles ? i : m0 + i - s_tiles) * kTileKeys; }
+
+// 2^x for a pair of exponents without the special-function unit: x = n + f with n = round(x), f in [-0.5, 0.5]; 2^f by the
+// cubic of least relative error (1.0e-4, a nineteenth of what rounding a weight to bf16 costs, a fifth for fp16) among
+// those that are 1 at 0 -- so that everything below 2^-127, -inf first of all, becomes 0 exactly -- and n added into the
+// exponent field (the magic constant 1.5 * 2^23 leaves it in the low bits).  A NaN comes out as 3.4e38, which the sums notice.
+__device__ __forceinline__ void exp2_pair(float x0, float x1, float& p0, float& p1) {
+  asm("min.NaN.xorsign.abs.f32 %0, %0, %1;" : "+f"(x0) : "f"(127.f));  // into [-127, 127]
+  asm("min.NaN.xorsign.abs.f32 %0, %0, %1;" : "+f"(x1) : "f"(127.f));
+  const uint64_t x = f2_pack(x0, x1), one = f2_pack(1.f, 1.f);
+  const uint64_t t2 = f2_add(x, f2_pack(12582912.f, 12582912.f));
+  const uint64_t n2 = f2_add(t2, f2_pack(-12582912.f, -12582912.f));
+  const uint64_t f2 = f2_fma(n2, f2_pack(-1.f, -1.f), x);
+  uint64_t q = f2_fma(f2_pack(0.0550090596f, 0.0550090596f), f2, f2_pack(0.242210969f, 0.242210969f));
+  q = f2_fma(q, f2, f2_pack(0.693282902f, 0.693282902f));
+  q = f2_fma(q, f2, one);
+  float q0, q1, t0, t1;
+  f2_unpack(q, q0, q1);
+  f2_unpack(t2, t0, t1);
+  p0 = __int_as_float(__float_as_int(q0) + (__float_as_int(t0) << 23));
+  p1 = __int_as_float(__float_as_int(q1) + (__float_as_int(t1) << 23));
+}
+
+// A row tile: rows [row0, row0 + 256) of the n * group (token, head) rows of a request under one KV head.
+struct RowTile {
+  int row0, rows;             // first row, rows of the request
+  TileList<kTileKeys> list;   // the cache tiles its rows see
+  int n;                      // at least one: a tile whose rows see nothing still writes its zeros
+  RowTile() = default;
+  __device__ __forceinline__ RowTile(const ChunkArgs& ka, const Request& rq, int qt)
+      : row0(qt * kCtaRows),
+        rows(rq.n * ka.group),
+        list(rq.first_pos + row0 / ka.group, rq.first_pos + (min(row0 + kCtaRows, rows) - 1) / ka.group, ka.a.window, ka.a.sinks) {
+    n = max(list.n, 1);
+  }
+  __device__ __forceinline__ int cost() const { return n + 1; }
+};
+__device__ __forceinline__ int row_tiles(const ChunkArgs& ka, const Request& rq) {
+  const int rows = rq.n * ka.group;
+  return rows > ka.few_rows ? (rows + kCtaRows - 1) / kCtaRows : 0;
+}
+
+// A place in the line: cache tile i of row tile qt of (request b, KV head h); b == batch: the end.
+struct Place {
+  int b, h, qt, i;
+};
+
+// What the requests of [b0, b1) cost under one KV head (a warp).
+__device__ long long requests_cost(const ChunkArgs& ka, int b0, int b1) {
+  const int lane = threadIdx.x & 31;
+  long long sum = 0;
+  for (int c0 = b0; c0 < b1; c0 += 32) {
+    const Request mine = c0 + lane < b1 ? read_request(ka.a, c0 + lane, false) : Request{};
+    uint32_t todo = __ballot_sync(0xffffffffu, row_tiles(ka, mine) > 0);
+    while (todo) {
+      const int src = __ffs(todo) - 1;
+      todo &= todo - 1;
+      const Request rq = shfl_request(mine, src);
+      const int nqt = row_tiles(ka, rq);
+      for (int qt = lane; qt < nqt; qt += 32) sum += RowTile(ka, rq, qt).cost();
+    }
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  return sum;
+}
+
+// The place `g` into the line (a warp).  Places inside short row tiles, or next to an edge, move to the edge: every CTA
+// finds the same.
+__device__ Place locate(const ChunkArgs& ka, long long g, const long long* group_cost, int group_size) {
+  const int lane = threadIdx.x & 31, H = ka.a.num_kv_heads;
+  int grp = 0;
+  while (grp < kGroups && g >= group_cost[grp] * H) g -= group_cost[grp++] * H;
+  Place at{ka.a.batch, 0, 0, 0};
+  if (grp == kGroups) return at;
+  for (int b = grp * group_size; b < min((grp + 1) * group_size, ka.a.batch); ++b) {
+    const long long cost = requests_cost(ka, b, b + 1);
+    if (g >= cost * H) {
+      g -= cost * H;
+      continue;
+    }
+    at.b = b;
+    at.h = (int)(g / cost);
+    g -= at.h * cost;
+    const Request rq = read_request(ka.a, b, false);
+    const int nqt = row_tiles(ka, rq);
+    for (int q0 = 0; q0 < nqt; q0 += 32) {
+      const RowTile tile(ka, rq, min(q0 + lane, nqt - 1));
+      int incl = q0 + lane < nqt ? tile.cost() : 0;
+      const int own = incl;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += o;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, incl > g);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        at.qt = q0 + src;
+        const int n = __shfl_sync(0xffffffffu, tile.n, src);
+        at.i = (int)(g - __shfl_sync(0xffffffffu, incl - own, src));
+        if (n <= kSnapTiles)
+          at.i = 2 * at.i < n ? 0 : n;
+        else if (at.i < 2 || at.i > n - 2)
+          at.i = at.i < 2 ? 0 : n;
+        if (at.i == n) {  // the next row tile's start
+          at.i = 0;
+          if (++at.qt == nqt) {
+            at.qt = 0;
+            if (++at.h == H) at.h = 0, ++at.b;
+          }
+        }
+        return at;
+      }
+      g -= __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+  at.b = ka.a.batch;  // (the groups' costs say that this does not happen)
+  return at;
+}
+
+// A piece: what a run has of one row tile.  Warp 9 walks the run and hands the pieces to the other warps through shared
+// memory (a walker of thirty words in every warp pushes the softmax's scores out of the registers).
+struct Piece {
+  int valid;                    // 0: the run is over
+  int b, h, q0, first_pos, kv_len;
+  int row0, rows;               // rows [row0, row0 + 256) of the request's
+  int i0, ntiles, whole;        // cache tiles [i0, i0 + ntiles) of the row tile's list; all of them?
+  int s_tiles, m0, hi, lo, snk;  // the list (TileList)
+};
+constexpr int kPieces = 4;  // in flight
+constexpr int kPieceReaders = 11;
+
+struct Pieces {
+  Place at, end;  // the run ends in front of `end`
+  Request rq;
+  RowTile tile;
+  int nqt, i0, ntiles;  // row tiles of the request; this piece's cache tiles [i0, i0 + ntiles) of the row tile's list
+  bool fresh;
+  __device__ __forceinline__ Pieces(const Place& from, const Place& to) : at(from), end(to), rq{}, nqt(0), i0(0), ntiles(0), fresh(true) {}
+  __device__ __forceinline__ bool next(const ChunkArgs& ka) {
+    if (fresh) {
+      request(ka);
+    } else if (++at.qt == nqt) {
+      at.qt = 0;
+      if (++at.h == ka.a.num_kv_heads) {
+        at.h = 0;
+        ++at.b;
+        request(ka);
+      }
+    }
+    if (at.b > end.b || at.b >= ka.a.batch) return false;
+    const bool in_last = at.b == end.b && at.h == end.h && at.qt == end.qt;
+    if (at.b == end.b && !in_last && (at.h > end.h || (at.h == end.h && at.qt > end.qt))) return false;
+    tile = RowTile(ka, rq, at.qt);
+    i0 = fresh ? at.i : 0;
+    fresh = false;
+    ntiles = (in_last ? end.i : tile.n) - i0;
+    return ntiles > 0;
+  }
+  __device__ __forceinline__ Piece piece(bool any) const {
+    return Piece{any, at.b, at.h, rq.q0, rq.first_pos, rq.kv_len, tile.row0, tile.rows, i0, ntiles, ntiles == tile.n,
+                 tile.list.s_tiles, tile.list.m0, tile.list.hi, tile.list.lo, tile.list.snk};
+  }
+
+ private:
+  __device__ __forceinline__ void request(const ChunkArgs& ka) {  // the next one with row tiles
+    for (nqt = 0; at.b < ka.a.batch && at.b <= end.b; ++at.b) {
+      rq = read_request(ka.a, at.b, false);
+      nqt = row_tiles(ka, rq);
+      if (nqt > 0) return;
+      at.h = at.qt = at.i = 0;
+    }
+  }
+};
+
 template <bool kHalf, int kDim>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     chunk_attn_tc_kernel(const ChunkArgs ka, const __grid_constant__ CUtensorMap tmap_k,
                          const __grid_constant__ CUtensorMap tmap_v) {
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t full[kRing], empty[kRing], s_ready[2], p_ready[2][2], o_done[2], q_ready, fix, drained;
+  __shared__ __align__(8) uint64_t full[kRing], empty[kRing], s_ready[2], p_ready[2][2], h_done[2], o_done[2], q_ready, fix, drained, pc_full[kPieces], pc_empty[kPieces];
+  __shared__ long long s_cost[kGroups];
+  __shared__ Place s_place[2];
+  __shared__ Piece s_piece[kPieces];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   constexpr int kHalves = kDim / 64;
@@ -74,85 +262,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   constexpr int kQHalfBytes = kBlockRows * 128;         // 64 dims of a Q block's rows
   constexpr int kQBlockBytes = kHalves * kQHalfBytes;
   const subspec_chunk_attn_args& a = ka.a;
-  const int kvh = blockIdx.y, G = ka.group;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = (int)blockIdx.x % ka.splits;
+  const int G = ka.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, run = (int)blockIdx.x;
   grid_dep_launch();
-
-  // ---- which request and which of its row tiles: every warp looks for itself ----
-  int b = -1, qt = 0;
-  Request rq{};
-  {
-    int rem = (int)blockIdx.x / ka.splits;
-    for (int b0 = 0; b0 < a.batch && b < 0; b0 += 32) {
-      Request r{};
-      int tiles = 0;
-      if (b0 + lane < a.batch) {
-        r = read_request(a, b0 + lane, false);
-        if (r.n * G > ka.few_rows) tiles = (r.n * G + kCtaRows - 1) / kCtaRows;
-      }
-      int incl = tiles;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += o;
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, incl > rem);
-      if (hit) {
-        const int src = __ffs(hit) - 1;
-        b = b0 + src;
-        qt = __shfl_sync(0xffffffffu, incl, src) - 1 - rem;  // the last row tile first: it has the most tiles
-        rq.q0 = __shfl_sync(0xffffffffu, r.q0, src);
-        rq.n = __shfl_sync(0xffffffffu, r.n, src);
-        rq.first_pos = __shfl_sync(0xffffffffu, r.first_pos, src);
-        rq.kv_len = __shfl_sync(0xffffffffu, r.kv_len, src);
-      } else {
-        rem -= __shfl_sync(0xffffffffu, incl, 31);
-      }
-    }
-  }
   // lengths that do not fit are reported once a launch
   auto report = [&]() {
-    if (blockIdx.x == 0 && kvh == 0)
+    if (run == 0)
       for (int x = lane; x < a.batch; x += 32) read_request(a, x, true);
   };
-  if (b < 0) {
-    if (warp == 0) report();
-    return;
-  }
-  const int rows = rq.n * G, row0 = qt * kCtaRows;
-  const int nblk = row0 + kBlockRows < rows ? 2 : 1;
-  // cache rows of a block's first and last token
-  auto block_pos = [&](int blk, int& first, int& last) {
-    first = rq.first_pos + (row0 + blk * kBlockRows) / G;
-    last = rq.first_pos + (min(row0 + (blk + 1) * kBlockRows, rows) - 1) / G;
-  };
-  int pmin, pmax, unused;
-  block_pos(0, pmin, pmax);
-  if (nblk == 2) block_pos(1, unused, pmax);
-  const TileList<kTileKeys> tiles(pmin, pmax, a.window, a.sinks);
-  const int per = per_split(tiles.n, ka.splits);
-  const int i0 = split * per, ntiles = min(per, tiles.n - i0);  // this CTA's part of the list
-  const bool partial = per < tiles.n;
-  if (ntiles <= 0 && split > 0) return;
-  if (ntiles <= 0) {  // nothing to attend to: zeros, as the sum of no terms
-    if (warp == 0) report();
-    const int row = row0 + (int)threadIdx.x;
-    if (threadIdx.x < kCtaRows && row < rows) {
-      uint4* o = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + (size_t)(rq.q0 + row / G) * a.o_token_stride +
-                                          (size_t)(kvh * G + row % G) * a.o_head_stride);
-      for (int c = 0; c < kDim / 8; ++c) o[c] = make_uint4(0u, 0u, 0u, 0u);
-    }
-    return;
-  }
-  // Whether a block's rows see anything of tile row t0, and whether all of them see all of it.
-  auto block_sees = [&](int first, int last, int t0) {
-    return t0 <= last && (a.window == 0 || t0 + kTileKeys - 1 > first - a.window || t0 < a.sinks);
-  };
-  auto block_sees_all = [&](int first, int last, int t0) {
-    return t0 + kTileKeys - 1 <= first && (a.window == 0 || t0 > last - a.window || t0 + kTileKeys <= a.sinks);
-  };
 
+  // ---- this CTA's run of the line ----
+  const int group_size = (a.batch + kGroups - 1) / kGroups;
+  for (int g = warp; g < kGroups; g += kChunkThreads / 32) {
+    const long long c = requests_cost(ka, min(g * group_size, a.batch), min((g + 1) * group_size, a.batch));
+    if (lane == 0) s_cost[g] = c;
+  }
   unsigned char* qtiles = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* ring = qtiles + 2 * kQBlockBytes;
   if (threadIdx.x == 0) {
@@ -164,13 +287,34 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       mbar_init(&s_ready[k], 1);
       mbar_init(&p_ready[k][0], 4);
       mbar_init(&p_ready[k][1], 4);
+      mbar_init(&h_done[k], 1);
       mbar_init(&o_done[k], 1);
     }
-    mbar_init(&q_ready, kCtaRows);
+    mbar_init(&q_ready, 8);
+    for (int k = 0; k < kPieces; ++k) {
+      mbar_init(&pc_full[k], 1);
+      mbar_init(&pc_empty[k], kPieceReaders);
+    }
     mbar_init(&fix, 1);
     mbar_init(&drained, 1);
     mbar_init_fence();
     s_abort = 0;
+  }
+  __syncthreads();
+  long long total = 0;
+  for (int g = 0; g < kGroups; ++g) total += s_cost[g];
+  total *= a.num_kv_heads;
+  const int runs = (int)max(1LL, min((long long)gridDim.x, total / kMinRun));
+  int4* record = ka.runs + run;
+  if (total == 0 || run >= runs) {
+    if (warp == 0) report();
+    if (threadIdx.x == 0) *record = make_int4(0, 0, 0, 0);
+    return;
+  }
+  if (warp < 2) {
+    const int c = run + warp;
+    const Place p = c < runs ? locate(ka, c * total / runs, s_cost, group_size) : Place{a.batch, 0, 0, 0};
+    if (lane == 0) s_place[warp] = p;
   }
   if (warp == kIssuerWarp) {
     tmem_alloc(&s_tmem, 512);
@@ -182,372 +326,477 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const uint32_t tmem = s_tmem;
   volatile int* abort_flag = &s_abort;
 
+  // Reading the pieces: peek waits for the next one, pop lets go of its slot.
+  int pc_slot = 0;
+  uint32_t pc_phase = 0;
+  auto peek = [&]() -> const Piece* {
+    const bool ok = __all_sync(0xffffffffu, tc_wait(&pc_full[pc_slot], pc_phase, abort_flag));
+    return ok && s_piece[pc_slot].valid ? &s_piece[pc_slot] : nullptr;
+  };
+  auto pop = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&pc_empty[pc_slot]);
+    if (++pc_slot == kPieces) pc_slot = 0, pc_phase ^= 1u;
+  };
+  // Rows of a block of a piece: cache rows of its first and last token; a block without rows sees nothing.
+  auto block_pos = [&](const Piece& pc, int blk, int& first, int& last) {
+    const int r0 = pc.row0 + blk * kBlockRows;
+    first = pc.first_pos + r0 / G;
+    last = r0 < pc.rows ? pc.first_pos + (min(r0 + kBlockRows, pc.rows) - 1) / G : -1;
+  };
+  // Whether a block's rows see anything of tile row t0, and whether all of them see all of it.
+  auto block_sees = [&](int first, int last, int t0) {
+    return t0 <= last && (a.window == 0 || t0 + kTileKeys - 1 > first - a.window || t0 < a.sinks);
+  };
+  auto block_sees_all = [&](int first, int last, int t0) {
+    return t0 + kTileKeys - 1 <= first && (a.window == 0 || t0 > last - a.window || t0 + kTileKeys <= a.sinks);
+  };
+
   if (warp < 8) {
     // ================= softmax =================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int blk = warp >> 2, rr = (int)threadIdx.x & 127;
-    const int row = row0 + (int)threadIdx.x;
-    const bool row_ok = row < rows;
-    const int tok = row / G, head = kvh * G + row - tok * G;
-    {  // every thread brings its own row of Q (a row that does not exist: zeros)
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)blk * kBlockCols;
+    const uint32_t o_addr = lane_base + kOCol;
+    const float c2 = ka.scale_log2;
+    const uint64_t c2p = f2_pack(c2, c2);
+    // fp16 weights sit 2^7 higher, out of the subnormals
+    constexpr float kOffset = kHalf ? 7.f : 0.f;
+    constexpr float kSumLimit = kHalf ? 32768.f : 1.0995116e12f;
+    uint32_t seen = 0, finished = 0;  // tiles, and pieces with any, that this block has worked on
+    // Every thread brings its own row of Q of a piece (a row that does not exist: zeros) ...
+    auto load_q = [&](const Piece& pc) {
+      const int row = pc.row0 + (int)threadIdx.x, tok = row / G;
+      const bool ok = row < pc.rows;
       const unsigned char* src = reinterpret_cast<const unsigned char*>(a.q);
-      if (row_ok) src += 2 * ((size_t)(rq.q0 + tok) * a.q_token_stride + (size_t)head * a.q_head_stride);
+      if (ok) src += 2 * ((size_t)(pc.q0 + tok) * a.q_token_stride + (size_t)(pc.h * G + row - tok * G) * a.q_head_stride);
       unsigned char* d = qtiles + blk * kQBlockBytes + rr * 128;
 #pragma unroll
       for (int c = 0; c < kDim / 8; ++c)
-        cp_async16(d + (c >> 3) * kQHalfBytes + (((c & 7) ^ (rr & 7)) << 4), src + c * 16, row_ok ? 16 : 0);
+        cp_async16(d + (c >> 3) * kQHalfBytes + (((c & 7) ^ (rr & 7)) << 4), src + c * 16, ok ? 16 : 0);
       cp_async_commit();
+    };
+    auto hand_q = [&]() {  // ... and the issuer may read it
       cp_async_wait<0>();
       fence_async_smem();
-      mbar_arrive(&q_ready);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_ready);
+    };
+    bool live = true;
+    if (const Piece* first = peek()) {
+      load_q(*first);
+      hand_q();
     }
-    if (blk < nblk) {
+    while (live) {
+      const Piece* now = peek();
+      if (!now) break;
+      const int row = now->row0 + (int)threadIdx.x;
+      const bool row_ok = row < now->rows, block_ok = now->row0 + blk * kBlockRows < now->rows, whole = now->whole;
+      const int tok = row / G, head = now->h * G + row - tok * G, t = now->q0 + tok, b = now->b;
       int bfirst, blast;
-      block_pos(blk, bfirst, blast);
-      const int pos = min(rq.first_pos + tok, blast);  // rows that do not exist look like the last one
-      const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)blk * kBlockCols;
-      const uint32_t o_addr = lane_base + kOCol;
-      const float c2 = ka.scale_log2;
-      // fp16 weights sit 2^7 higher, out of the subnormals: at most 2^(7 + 8) between moves of the reference point
-      constexpr float kOffset = kHalf ? 7.f : 0.f;
+      block_pos(*now, blk, bfirst, blast);
+      const int pos = min(now->first_pos + tok, blast);  // rows that do not exist look like the last one
+      const int ntiles = now->ntiles, i0 = now->i0, s_tiles = now->s_tiles, m0 = now->m0;
+      pop();
       float m = -INFINITY, l = 0.f;
-      uint32_t done = 0;  // tiles this block has worked on
-      bool live = true;
+      uint32_t done = 0;  // tiles of this piece
       for (int i = 0; i < ntiles; ++i) {
-        const int t0 = tiles.first_row(i0 + i);
+        const int t0 = list_row(s_tiles, m0, i0 + i);
         if (!block_sees(bfirst, blast, t0)) continue;
-        live = __all_sync(0xffffffffu, tc_wait(&s_ready[blk], done & 1u, abort_flag));
+        live = __all_sync(0xffffffffu, tc_wait(&s_ready[blk], seen & 1u, abort_flag));
         if (!live) break;
         tc_fence_after();
         uint32_t r[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32_async(lane_base + 32 * c, r[c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_wait_ld_dep(r[c]);
+        tmem_ld32_async(lane_base, r[0]);
+        tmem_ld32_async(lane_base + 32, r[1]);
+        tmem_wait_ld_dep(r[0]);
+        tmem_wait_ld_dep(r[1]);
+        tmem_ld32_async(lane_base + 64, r[2]);
+        tmem_ld32_async(lane_base + 96, r[3]);
         const bool masked = !block_sees_all(bfirst, blast, t0);
-        if (masked) {
+        auto hide = [&](int c) {
+          const int p0 = t0 + 32 * c;
+          uint32_t bits = bits_below(pos + 1 - p0);
+          if (a.window > 0) bits &= ~bits_below(pos - a.window + 1 - p0) | bits_below(a.sinks - p0);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int p0 = t0 + 32 * c;
-            uint32_t bits = bits_below(pos + 1 - p0);
-            if (a.window > 0) bits &= ~bits_below(pos - a.window + 1 - p0) | bits_below(a.sinks - p0);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) r[c][j] = (bits >> j) & 1u ? r[c][j] : 0xff800000u;
-          }
-        }
-        // the row's maximum over the tile; NaN stays NaN (a NaN score makes the row NaN)
-        float mx[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          mx[c] = max3_nan(__uint_as_float(r[c][0]), __uint_as_float(r[c][1]), __uint_as_float(r[c][2]));
-#pragma unroll
-          for (int j = 3; j < 31; j += 2) mx[c] = max3_nan(mx[c], __uint_as_float(r[c][j]), __uint_as_float(r[c][j + 1]));
-          mx[c] = max3_nan(mx[c], __uint_as_float(r[c][31]), mx[c]);
-        }
-        const float tmax = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * c2;  // c2 > 0
-        float alpha = 1.f;
-        if (!(tmax <= m + kRescaleAt) || m == -INFINITY) {
-          const float m_new = max3_nan(m, tmax, tmax);
-          alpha = m == -INFINITY ? 0.f : ex2f(m - m_new);
-          m = m_new;
-        }
-        if (done > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-          // O is complete up to the tile before: its MMAs were committed together with this tile's scores
-#pragma unroll
-          for (int c = 0; c < kDim / 32; ++c) {
-            uint32_t rc[32];
-            tmem_ld32_async(o_addr + 32 * c, rc);
-            tmem_wait_ld_dep(rc);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) rc[j] = __float_as_uint(__uint_as_float(rc[j]) * alpha);
-            tmem_st32(o_addr + 32 * c, rc);
-          }
-        }
-        const float u = m == -INFINITY ? 0.f : m - kOffset;  // (-inf: nothing seen yet, every weight 0)
-        uint64_t sm2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-        const uint64_t c2p = f2_pack(c2, c2), nup = f2_pack(-u, -u);
-        auto exp_tile = [&](auto plain) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float x0, x1, p0, p1;
-              f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c][2 * j]), __uint_as_float(r[c][2 * j + 1])), c2p, nup), x0, x1);
-              if (decltype(plain)::value && ((j & 3) == 3 || (j & 7) == 1)) {
-                exp2_pair_fma(x0, x1, p0, p1);  // three pairs in eight on the FMA pipe
-              } else {
-                p0 = ex2f(x0);  // 2^-inf = 0: hidden entries get the weight 0 exactly
-                p1 = ex2f(x1);
-              }
-              sm2[j & 1] = f2_add(sm2[j & 1], f2_pack(p0, p1));
-              pk[j] = pack16<kHalf>(p0, p1);
-            }
-            tmem_st16(lane_base + 16 * c, pk);
-            if (c & 1) {  // half of the tile: its share of O += P V can begin
-              tmem_wait_st();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&p_ready[blk][c >> 1]);
-            }
-          }
+          for (int j = 0; j < 32; ++j) r[c][j] = (bits >> j) & 1u ? r[c][j] : 0xff800000u;
         };
-        if (masked)
-          exp_tile(std::false_type{});
-        else
-          exp_tile(std::true_type{});
-        float e0, e1, e2, e3;
-        f2_unpack(sm2[0], e0, e1);
-        f2_unpack(sm2[1], e2, e3);
-        l = l * alpha + ((e0 + e1) + (e2 + e3));
-        ++done;
-      }
-      // ---- the result: O / l ----
-      if (live && done > 0) live = __all_sync(0xffffffffu, tc_wait(&o_done[blk], 0, abort_flag));
-      if (live) {
-        tc_fence_after();
-        const float inv = l != 0.f ? 1.f / l : 0.f;
-        bool odd = false;  // a value that is not finite although the sum of the weights is
-        const size_t prow = ((size_t)(rq.q0 + tok) * a.num_q_heads + head) * ka.splits + split;
-        uint16_t* out_row = reinterpret_cast<uint16_t*>(a.out) + (size_t)(rq.q0 + tok) * a.o_token_stride +
-                            (size_t)head * a.o_head_stride;
-        if (partial && row_ok) {
-          ka.part_ml[prow * 2] = m;
-          ka.part_ml[prow * 2 + 1] = l;
-        }
+        auto max32 = [&](int c) {  // NaN stays NaN: a NaN score makes the row NaN
+          float mx[2] = {__uint_as_float(r[c][0]), __uint_as_float(r[c][1])};
 #pragma unroll
-        for (int c = 0; c < kDim / 32; ++c) {
-          uint32_t rc[32];
-          if (done > 0) {
-            tmem_ld32_async(o_addr + 32 * c, rc);
-            tmem_wait_ld_dep(rc);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) rc[j] = 0u;
+          for (int j = 2; j < 30; j += 4) {
+            mx[0] = max3_nan(mx[0], __uint_as_float(r[c][j]), __uint_as_float(r[c][j + 1]));
+            mx[1] = max3_nan(mx[1], __uint_as_float(r[c][j + 2]), __uint_as_float(r[c][j + 3]));
           }
-          if (partial) {
-            if (row_ok) {
+          mx[0] = max3_nan(mx[0], __uint_as_float(r[c][30]), __uint_as_float(r[c][31]));
+          return max3_nan(mx[0], mx[1], mx[1]) * c2;  // c2 > 0
+        };
+        // Weights need a reference point near the row's maximum, not the maximum itself: a tile is first tried against the
+        // old one, without looking for its maximum.  Every weight is positive, so a sum within kSumLimit proves that none
+        // is too large (for the 16-bit type and the fp32 sums); anything else (a larger sum, an overflow, NaN, a row that
+        // has seen nothing yet) moves the reference point to the maximum, rescales O and does the half tile again.
+        bool rest = false;  // the second half of the scores has arrived
+        auto arrive_rest = [&]() {
+          if (rest) return;
+          rest = true;
+          tmem_wait_ld_dep(r[2]);
+          tmem_wait_ld_dep(r[3]);
+          if (masked) hide(2), hide(3);
+        };
+        if (masked) hide(0), hide(1);
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                reinterpret_cast<uint4*>(ka.part_o + prow * kDim)[8 * c + j] =
-                    make_uint4(rc[4 * j], rc[4 * j + 1], rc[4 * j + 2], rc[4 * j + 3]);
+        for (int half = 0; half < 2; ++half) {
+          if (half == 1) arrive_rest();
+          bool move = half == 0 && m == -INFINITY, moved = false;
+          uint32_t pk[2][16];
+          float sum;
+          for (;;) {
+            if (__any_sync(0xffffffffu, move)) {
+              moved = true;
+              float alpha = 1.f;
+              arrive_rest();
+              float top = max3_nan(max32(2), max32(3), m);
+              if (half == 0) top = max3_nan(max32(0), max32(1), top);
+              if (move) {
+                alpha = m == -INFINITY ? 0.f : ex2f(m - top);
+                m = top;
+              }
+              if (half == 1) {  // O is at rest only when the first half's MMAs have landed
+                live = __all_sync(0xffffffffu, tc_wait(&h_done[blk], seen & 1u, abort_flag));
+                tc_fence_after();
+              }
+              if ((done > 0 || half == 1) && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+                for (int c = 0; c < kDim / 32; ++c) {
+                  uint32_t rc[32];
+                  tmem_ld32_async(o_addr + 32 * c, rc);
+                  tmem_wait_ld_dep(rc);
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) rc[j] = __float_as_uint(__uint_as_float(rc[j]) * alpha);
+                  tmem_st32(o_addr + 32 * c, rc);
+                }
+              }
+              l *= alpha;
             }
-          } else {
+            const float u = m == -INFINITY ? 0.f : m - kOffset;  // (-inf: every score is -inf, every weight 0)
+            const uint64_t nup = f2_pack(-u, -u);
+            uint64_t sm2[4] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f), f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float x = pos < 0 ? 0.f : __uint_as_float(rc[j]) * inv;
-              odd = odd || !(fabsf(x) < INFINITY);
-              rc[j] = __float_as_uint(x);
-            }
-            if (row_ok) {
+            for (int c = 0; c < 2; ++c) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                uint4 v;
-                v.x = pack16<kHalf>(__uint_as_float(rc[8 * j]), __uint_as_float(rc[8 * j + 1]));
-                v.y = pack16<kHalf>(__uint_as_float(rc[8 * j + 2]), __uint_as_float(rc[8 * j + 3]));
-                v.z = pack16<kHalf>(__uint_as_float(rc[8 * j + 4]), __uint_as_float(rc[8 * j + 5]));
-                v.w = pack16<kHalf>(__uint_as_float(rc[8 * j + 6]), __uint_as_float(rc[8 * j + 7]));
-                reinterpret_cast<uint4*>(out_row)[4 * c + j] = v;
+              for (int j = 0; j < 16; ++j) {
+                const uint32_t* s = &r[2 * half + c][2 * j];
+                float x0, x1, p0, p1;
+                f2_unpack(f2_fma(f2_pack(__uint_as_float(s[0]), __uint_as_float(s[1])), c2p, nup), x0, x1);
+                if (j % kFmaEvery == kFmaEvery - 1) {
+                  exp2_pair(x0, x1, p0, p1);  // some pairs on the FMA pipe
+                } else {
+                  p0 = ex2f(x0);
+                  p1 = ex2f(x1);
+                }
+                sm2[j & 3] = f2_add(sm2[j & 3], f2_pack(p0, p1));
+                pk[c][j] = pack16<kHalf>(p0, p1);
               }
             }
+            float e0, e1;
+            f2_unpack(f2_add(f2_add(sm2[0], sm2[1]), f2_add(sm2[2], sm2[3])), e0, e1);
+            sum = e0 + e1;
+            move = !(sum <= kSumLimit);
+            if (moved || !__any_sync(0xffffffffu, move)) break;
+          }
+          l += sum;
+          tmem_st16(lane_base + 32 * half, pk[0]);
+          tmem_st16(lane_base + 32 * half + 16, pk[1]);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_ready[blk][half]);  // this half's share of O += P V can begin
+        }
+        if (!live) break;
+        ++done;
+        ++seen;
+      }
+      // The block's Q has served its last scores: the next piece's comes while the last MMAs run.
+      const Piece* following = live ? peek() : nullptr;
+      if (following) load_q(*following);
+      // ---- the result: O / l, or the part as it is ----
+      if (live && done > 0) live = __all_sync(0xffffffffu, tc_wait(&o_done[blk], finished++ & 1u, abort_flag));
+      if (following) hand_q();
+      if (!live) break;
+      if (!block_ok) continue;
+      tc_fence_after();
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+      bool odd = false;  // a value that is not finite although the sum of the weights is
+      const size_t prow = ((size_t)2 * run + (i0 == 0 ? 1 : 0)) * kCtaRows + threadIdx.x;
+      uint16_t* out_row = reinterpret_cast<uint16_t*>(a.out) + (size_t)t * a.o_token_stride + (size_t)head * a.o_head_stride;
+      if (!whole && row_ok) reinterpret_cast<float2*>(ka.part_ml)[prow] = make_float2(m, l);
+#pragma unroll
+      for (int c = 0; c < kDim / 32; ++c) {
+        uint32_t rc[32];
+        if (done > 0) {
+          tmem_ld32_async(o_addr + 32 * c, rc);
+          tmem_wait_ld_dep(rc);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) rc[j] = 0u;
+        }
+        if (!whole) {
+          if (row_ok) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              reinterpret_cast<uint4*>(ka.part_o + prow * kDim)[8 * c + j] =
+                  make_uint4(rc[4 * j], rc[4 * j + 1], rc[4 * j + 2], rc[4 * j + 3]);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float x = pos < 0 ? 0.f : __uint_as_float(rc[j]) * inv;
+            odd = odd || !(fabsf(x) < INFINITY);
+            rc[j] = __float_as_uint(x);
+          }
+          if (row_ok) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint4 v;
+              v.x = pack16<kHalf>(__uint_as_float(rc[8 * j]), __uint_as_float(rc[8 * j + 1]));
+              v.y = pack16<kHalf>(__uint_as_float(rc[8 * j + 2]), __uint_as_float(rc[8 * j + 3]));
+              v.z = pack16<kHalf>(__uint_as_float(rc[8 * j + 4]), __uint_as_float(rc[8 * j + 5]));
+              v.w = pack16<kHalf>(__uint_as_float(rc[8 * j + 6]), __uint_as_float(rc[8 * j + 7]));
+              reinterpret_cast<uint4*>(out_row)[4 * c + j] = v;
+            }
           }
         }
-        tc_fence_before();
-        // 0 * inf from a V row that this row does not see but others of the tile do, or scores of -inf alone: such
-        // rows are done over key by key.  (A NaN sum comes from scores the row sees: NaN is the result.)
-        uint32_t again = __ballot_sync(0xffffffffu, !partial && row_ok && l == l && (odd || (l == 0.f && pos >= 0)));
-        while (again) {
-          const int src = __ffs(again) - 1;
-          again &= again - 1;
-          attn_row<kHalf, kDim>(ka, b, __shfl_sync(0xffffffffu, pos, src), rq.q0 + __shfl_sync(0xffffffffu, tok, src),
-                                __shfl_sync(0xffffffffu, head, src), reinterpret_cast<float*>(qtiles + blk * kQBlockBytes) + (warp & 3) * kDim);
-        }
+      }
+      tc_fence_before();
+      // 0 * inf from a V row that this row does not see but others of the tile do, or scores of -inf alone: such rows
+      // are done over key by key.  (A NaN sum comes from scores the row sees: NaN is the result.)
+      uint32_t again = __ballot_sync(0xffffffffu, whole && row_ok && l == l && (odd || (l == 0.f && pos >= 0)));
+      while (again) {
+        const int src = __ffs(again) - 1;
+        again &= again - 1;
+        attn_row<kHalf, kDim>(ka, b, __shfl_sync(0xffffffffu, pos, src), __shfl_sync(0xffffffffu, t, src),
+                              __shfl_sync(0xffffffffu, head, src));
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp < kLoadWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == kIssuerWarp) {
       // ================= MMA issue: one warp for both blocks, an elected lane issues =================
       // One issuer, one block after the other: with an issuer per block the two blocks' MMAs interleave, both get
       // their scores at the same time and then both sit in their softmax while the tensor cores idle (4660 cycles a
       // tile against 2048 of MMAs).
-      if (warp == kIssuerWarp) {
-        constexpr uint32_t idesc_s = tc_idesc(kBlockRows, kTileKeys, false, kHalf);
-        constexpr uint32_t idesc_o = tc_idesc(kBlockRows, kDim, true, kHalf);
-        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        const uint32_t q_u32 = smem_u32(qtiles), ring_u32 = smem_u32(ring);
+      constexpr uint32_t idesc_s = tc_idesc(kBlockRows, kTileKeys, false, kHalf);
+      constexpr uint32_t idesc_o = tc_idesc(kBlockRows, kDim, true, kHalf);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t q_u32 = smem_u32(qtiles), ring_u32 = smem_u32(ring);
+      auto issue_s = [&](int blk, uint32_t tile) {
+#pragma unroll
+        for (int ks = 0; ks < kDim / 16; ++ks)
+          tc_mma_f16_ss(tm + (uint32_t)blk * kBlockCols,
+                        tc_desc(q_u32 + (uint32_t)(blk * kQBlockBytes + (ks >> 2) * kQHalfBytes + (ks & 3) * 32), 16),
+                        tc_desc(tile + (uint32_t)((ks >> 2) * 1024 + (ks & 3) * 32), 16, kGroupBytes), idesc_s, ks > 0 ? 1u : 0u);
+        tc_commit(&s_ready[blk]);
+      };
+      auto issue_o = [&](int blk, int half, uint32_t tile, bool accumulate) {
+#pragma unroll
+        for (int x = 0; x < kTileKeys / 32; ++x) {
+          const int ks = half * (kTileKeys / 32) + x;
+          tc_mma_f16_ta(tm + (uint32_t)blk * kBlockCols + kOCol, tm + (uint32_t)blk * kBlockCols + (uint32_t)(8 * ks),
+                        tc_desc(tile + (uint32_t)(ks * 2 * kGroupBytes), 1024, kGroupBytes), idesc_o, (accumulate || ks > 0) ? 1u : 0u);
+        }
+      };
+      // (A wait that gave up is noticed at the end of the tile: what is issued until then works on old data in bounds.)
+      bool ok = true, issued = false;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        ok = tc_wait(bar, parity, abort_flag) && ok;
+        __syncwarp();
+        tc_fence_after();
+      };
+      int e = 0;        // ring entry, in the order they come: K(0), V(0), K(1), ...
+      uint32_t ph = 0;  // and its phase
+      auto next_entry = [&]() {
+        if (++e == kRing) e = 0, ph ^= 1u;
+      };
+      uint32_t seen[2] = {0, 0}, piece = 0;
+      for (; ok; ++piece) {
+        const Piece* now = peek();
+        if (!now) break;
+        const int n = now->ntiles, i0 = now->i0, s_tiles = now->s_tiles, m0 = now->m0;
         int bfirst[2], blast[2], last_seen[2] = {-1, -1};
-        uint32_t done[2] = {0, 0};
-        block_pos(0, bfirst[0], blast[0]);
-        block_pos(nblk - 1, bfirst[1], blast[1]);
-        auto sees = [&](int blk, int i) { return blk < nblk && block_sees(bfirst[blk], blast[blk], tiles.first_row(i0 + i)); };
+        bool begun[2] = {false, false};
+        block_pos(*now, 0, bfirst[0], blast[0]);
+        block_pos(*now, 1, bfirst[1], blast[1]);
+        pop();
+        auto sees = [&](int blk, int i) { return block_sees(bfirst[blk], blast[blk], list_row(s_tiles, m0, i0 + i)); };
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk)
-          for (int i = ntiles - 1; i >= 0 && last_seen[blk] < 0; --i)
+          for (int i = n - 1; i >= 0 && last_seen[blk] < 0; --i)
             if (sees(blk, i)) last_seen[blk] = i;
-        auto issue_s = [&](int blk, uint32_t tile) {
+        wait(&q_ready, piece & 1u);
+        wait(&full[e], ph);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < kDim / 16; ++ks)
-            tc_mma_f16_ss(tm + (uint32_t)blk * kBlockCols,
-                          tc_desc(q_u32 + (uint32_t)(blk * kQBlockBytes + (ks >> 2) * kQHalfBytes + (ks & 3) * 32), 16),
-                          tc_desc(tile + (uint32_t)((ks >> 2) * 1024 + (ks & 3) * 32), 16, kGroupBytes), idesc_s, ks > 0 ? 1u : 0u);
-          tc_commit(&s_ready[blk]);
-        };
-        auto issue_o = [&](int blk, int half, uint32_t tile) {
-#pragma unroll
-          for (int x = 0; x < kTileKeys / 32; ++x) {
-            const int ks = half * (kTileKeys / 32) + x;
-            tc_mma_f16_ta(tm + (uint32_t)blk * kBlockCols + kOCol, tm + (uint32_t)blk * kBlockCols + (uint32_t)(8 * ks),
-                          tc_desc(tile + (uint32_t)(ks * 2 * kGroupBytes), 1024, kGroupBytes), idesc_o, (done[blk] > 0 || ks > 0) ? 1u : 0u);
-          }
-        };
-        auto wait = [&](uint64_t* bar, uint32_t parity) {
-          const bool ok = __all_sync(0xffffffffu, tc_wait(bar, parity, abort_flag));
-          tc_fence_after();
-          return ok;
-        };
-        int e = 0;        // ring entry, in the order they come: K(0), V(0), K(1), ...
-        uint32_t ph = 0;  // and its phase
-        auto next = [&]() {
-          if (++e == kRing) e = 0, ph ^= 1u;
-        };
-        bool issued = false;
-        bool ok = wait(&q_ready, 0) && wait(&full[0], 0);
-        if (ok) {
-          if (elect_one()) {
-#pragma unroll
-            for (int blk = 0; blk < 2; ++blk)
-              if (sees(blk, 0)) issue_s(blk, ring_u32);
-            tc_commit(&empty[0]);
-          }
-          __syncwarp();
-          issued = true;
-          next();
+          for (int blk = 0; blk < 2; ++blk)
+            if (sees(blk, 0)) issue_s(blk, ring_u32 + (uint32_t)(e * kTileBytes));
+          tc_commit(&empty[e]);
         }
-        for (int i = 0; i < ntiles && ok; ++i) {
+        __syncwarp();
+        issued = true;
+        next_entry();
+        for (int i = 0; i < n && ok; ++i) {
           const int ve = e;
-          ok = wait(&full[ve], ph);
-          next();
+          wait(&full[ve], ph);
+          next_entry();
           const int ke = e;
-          if (ok && i + 1 < ntiles) ok = wait(&full[ke], ph);
-          if (!ok) break;
+          const bool more = i + 1 < n;
           const uint32_t v_tile = ring_u32 + (uint32_t)(ve * kTileBytes), k_tile = ring_u32 + (uint32_t)(ke * kTileBytes);
 #pragma unroll
           for (int blk = 0; blk < 2; ++blk) {
             if (sees(blk, i)) {
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
-                if (!ok || !(ok = wait(&p_ready[blk][half], done[blk] & 1u))) break;
+                wait(&p_ready[blk][half], seen[blk] & 1u);
                 if (elect_one()) {
-                  issue_o(blk, half, v_tile);
+                  issue_o(blk, half, v_tile, begun[blk]);
+                  if (half == 0) tc_commit(&h_done[blk]);
                   if (half == 1 && i == last_seen[blk]) tc_commit(&o_done[blk]);
                 }
                 __syncwarp();
               }
-              if (!ok) break;
-              ++done[blk];
+              ++seen[blk];
+              begun[blk] = true;
             }
-            if (i + 1 < ntiles && sees(blk, i + 1)) {  // over the P just consumed: the MMAs of a thread run in order
+            if (blk == 0 && more) wait(&full[ke], ph);
+            if (more && sees(blk, i + 1)) {  // over the P just consumed: the MMAs of a thread run in order
               if (elect_one()) issue_s(blk, k_tile);
               __syncwarp();
             }
           }
-          if (!ok) break;
           if (elect_one()) {
             tc_commit(&empty[ve]);
-            if (i + 1 < ntiles) tc_commit(&empty[ke]);
+            if (more) tc_commit(&empty[ke]);
           }
           __syncwarp();
-          if (i + 1 < ntiles) next();
+          if (more) next_entry();
+          ok = __all_sync(0xffffffffu, ok);
         }
-        if (!ok && issued) {  // gave up: let the MMAs in flight finish before tensor memory is freed
-          if (elect_one()) tc_commit(&drained);
-          __syncwarp();
-          mbar_wait_bounded(&drained, 0);
+      }
+      if (!ok && issued) {  // gave up: let the MMAs in flight finish before tensor memory is freed
+        if (elect_one()) tc_commit(&drained);
+        __syncwarp();
+        mbar_wait_bounded(&drained, 0);
+      }
+    } else if (warp == kPieceWarp) {
+      // ================= the pieces of the run =================
+      Pieces pc(s_place[0], s_place[1]);
+      uint32_t ph = 1;  // the first round finds the slots empty
+      bool first = true, any = true;
+      for (int slot = 0; any; first = false) {
+        any = pc.next(ka);
+        if (!tc_wait(&pc_empty[slot], ph, abort_flag)) break;
+        if (lane == 0) {
+          s_piece[slot] = pc.piece(any);
+          mbar_arrive(&pc_full[slot]);
+          // what the join needs: the run's first row tile, whether it began in an earlier run, whether it ends in this one
+          if (first)
+            *record = make_int4(pc.at.b, pc.at.h, pc.at.qt,
+                                any ? (pc.i0 > 0 ? 1 : 0) | (pc.i0 + pc.ntiles == pc.tile.n ? 2 : 0) : 0);
         }
+        __syncwarp();
+        if (++slot == kPieces) slot = 0, ph ^= 1u;
       }
     } else {
       // ================= K (warp 10) and V (warp 11) tiles =================
       const int is_v = warp - kLoadWarp;
       const CUtensorMap* map = is_v ? &tmap_v : &tmap_k;
-      const unsigned char* base = (is_v ? ka.v_base : ka.k_base) + (size_t)kvh * kDim * 2;
-      const int* table = a.page_table + (size_t)b * a.pages_per_seq;
       const int box = ka.box_rows, boxes = box > 0 ? kTileKeys / box : 0;
       const int chunk = lane % (kDim / 8), sub = lane / (kDim / 8);  // row-by-row copies
       constexpr int kRowsPerPass = 32 / (kDim / 8);
       int e = is_v;
-      uint32_t ph = 1;  // the first round finds the entries empty
-      // rows some token of this CTA sees
-      auto wanted = [&](int lo, int hi) { return lo < tiles.hi && (hi > tiles.lo || lo < tiles.snk); };
-      auto page_of = [&](int i) -> int {  // what this lane's copy of tile i reads; -2: nothing (zeros)
-        if (lane >= boxes || i >= ntiles) return -2;
-        const int kpos = tiles.first_row(i0 + i) + lane * box;
-        if (!wanted(kpos, kpos + box)) return -2;
-        return table[ka.page_shift >= 0 ? kpos >> ka.page_shift : kpos / a.page_len];
-      };
-      int page = page_of(0);
-      for (int i = 0; i < ntiles; ++i) {
-        const int next = page_of(i + 1);  // asked for a tile ahead: a trip to memory
-        if (!tc_wait(&empty[e], ph, abort_flag)) break;
-        const int t0 = tiles.first_row(i0 + i);
-        unsigned char* dst = ring + (size_t)e * kTileBytes;
-        if (boxes > 0) {
-          // rows behind the cache's end, in a box with rows in front of it: whatever the page holds there must not
-          // meet a weight of 0 in the V tile
-          const int z0 = rq.kv_len - t0, z1 = min((rq.kv_len + box - 1) / box * box - t0, kTileKeys);
-          const bool tail = is_v && z0 > 0 && z0 < z1 && wanted(t0 + z1 - box, t0 + z0);
-          uint64_t* bar = tail ? &fix : &full[e];
-          if (lane == 0) mbar_expect_tx(bar, (uint32_t)kTileBytes);
-          __syncwarp();
-          if (lane < boxes) {
-            const int kpos = t0 + lane * box;
-            int unit = ka.units, slot = 0;  // outside the tensor: zeros, no memory is touched
-            if (page >= 0 && page < a.num_pages) {
-              unit = page * ka.page_units + kvh;
-              slot = ka.page_shift >= 0 ? kpos & (a.page_len - 1) : kpos % a.page_len;
-            } else if (page != -2) {
-              flag(a.dev_status, SUBSPEC_DEV_BAD_PAGE);
+      uint32_t ph = 1, fixes = 0;  // the first round finds the entries empty
+      bool live = true;
+      while (live) {
+        const Piece* now = peek();
+        if (!now) break;
+        const int ntiles = now->ntiles, i0 = now->i0, kv_len = now->kv_len, head = now->h;
+        const int s_tiles = now->s_tiles, m0 = now->m0, rows_hi = now->hi, rows_lo = now->lo, rows_snk = now->snk;
+        const unsigned char* base = (is_v ? ka.v_base : ka.k_base) + (size_t)head * kDim * 2;
+        const int* table = a.page_table + (size_t)now->b * a.pages_per_seq;
+        pop();
+        // rows some token of the row tile sees
+        auto wanted = [&](int lo, int hi) { return lo < rows_hi && (hi > rows_lo || lo < rows_snk); };
+        auto page_of = [&](int i) -> int {  // what this lane's copy of tile i reads; -2: nothing (zeros)
+          if (lane >= boxes || i >= ntiles) return -2;
+          const int kpos = list_row(s_tiles, m0, i0 + i) + lane * box;
+          if (!wanted(kpos, kpos + box)) return -2;
+          return table[ka.page_shift >= 0 ? kpos >> ka.page_shift : kpos / a.page_len];
+        };
+        int page = page_of(0);
+        for (int i = 0; i < ntiles; ++i) {
+          const int next = page_of(i + 1);  // asked for a tile ahead: a trip to memory
+          if (!(live = tc_wait(&empty[e], ph, abort_flag))) break;
+          const int t0 = list_row(s_tiles, m0, i0 + i);
+          unsigned char* dst = ring + (size_t)e * kTileBytes;
+          if (boxes > 0) {
+            // rows behind the cache's end, in a box with rows in front of it: whatever the page holds there must not
+            // meet a weight of 0 in the V tile
+            const int z0 = kv_len - t0, z1 = min((kv_len + box - 1) / box * box - t0, kTileKeys);
+            const bool tail = is_v && z0 > 0 && z0 < z1 && wanted(t0 + z1 - box, t0 + z0);
+            uint64_t* bar = tail ? &fix : &full[e];
+            if (lane == 0) mbar_expect_tx(bar, (uint32_t)kTileBytes);
+            __syncwarp();
+            if (lane < boxes) {
+              const int kpos = t0 + lane * box;
+              int unit = ka.units, slot = 0;  // outside the tensor: zeros, no memory is touched
+              if (page >= 0 && page < a.num_pages) {
+                unit = page * ka.page_units + head;
+                slot = ka.page_shift >= 0 ? kpos & (a.page_len - 1) : kpos % a.page_len;
+              } else if (page != -2) {
+                flag(a.dev_status, SUBSPEC_DEV_BAD_PAGE);
+              }
+              tma_load_5d(dst + (size_t)lane * box * kDim * 2, map, slot >> 3, unit, bar);
             }
-            tma_load_5d(dst + (size_t)lane * box * kDim * 2, map, slot >> 3, unit, bar);
-          }
-          if (tail) {
-            if (!tc_wait(&fix, 0, abort_flag)) break;
-            for (int x = lane; x < (z1 - z0) * (kDim / 8); x += 32) {
-              const int rr = z0 + x / (kDim / 8), c = x % (kDim / 8);
-              *reinterpret_cast<uint4*>(dst + (rr >> 3) * kGroupBytes + (c >> 3) * 1024 + (rr & 7) * 128 + ((c & 7) << 4)) =
-                  make_uint4(0u, 0u, 0u, 0u);
+            if (tail) {
+              if (!(live = tc_wait(&fix, fixes++ & 1u, abort_flag))) break;
+              for (int x = lane; x < (z1 - z0) * (kDim / 8); x += 32) {
+                const int rr = z0 + x / (kDim / 8), c = x % (kDim / 8);
+                *reinterpret_cast<uint4*>(dst + (rr >> 3) * kGroupBytes + (c >> 3) * 1024 + (rr & 7) * 128 + ((c & 7) << 4)) =
+                    make_uint4(0u, 0u, 0u, 0u);
+              }
+              fence_async_smem();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&full[e]);
             }
+          } else {
+            // a page length that is no multiple of 8: 16-byte copies, row by row
+  #pragma unroll 4
+            for (int pass = 0; pass < kTileKeys / kRowsPerPass; ++pass) {
+              const int rr = pass * kRowsPerPass + sub, kpos = t0 + rr;
+              const unsigned char* src = base;
+              int bytes = 0;
+              if (kpos < kv_len && wanted(kpos, kpos + 1)) {
+                const int pi = kpos / a.page_len, pg = table[pi];
+                if (pg < 0 || pg >= a.num_pages) {
+                  flag(a.dev_status, SUBSPEC_DEV_BAD_PAGE);
+                } else {
+                  bytes = 16;
+                  src = base + (size_t)pg * ka.page_stride + (size_t)(kpos - pi * a.page_len) * ka.row_stride + chunk * 16;
+                }
+              }
+              cp_async16(dst + (rr >> 3) * kGroupBytes + (chunk >> 3) * 1024 + (rr & 7) * 128 + (((chunk & 7) ^ (rr & 7)) << 4), src,
+                         bytes);
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[e]);
           }
-        } else {
-          // a page length that is no multiple of 8: 16-byte copies, row by row
-#pragma unroll 4
-          for (int pass = 0; pass < kTileKeys / kRowsPerPass; ++pass) {
-            const int rr = pass * kRowsPerPass + sub, kpos = t0 + rr;
-            const unsigned char* src = base;
-            int bytes = 0;
-            if (kpos < rq.kv_len && wanted(kpos, kpos + 1)) {
-              const int pi = kpos / a.page_len, pg = table[pi];
-              if (pg < 0 || pg >= a.num_pages) {
-                flag(a.dev_status, SUBSPEC_DEV_BAD_PAGE);
-              } else {
-                bytes = 16;
-                src = base + (size_t)pg * ka.page_stride + (size_t)(kpos - pi * a.page_len) * ka.row_stride + chunk * 16;
-              }
-            }
-            cp_async16(dst + (rr >> 3) * kGroupBytes + (chunk >> 3) * 1024 + (rr & 7) * 128 + (((chunk & 7) ^ (rr & 7)) << 4), src,
-                       bytes);
-          }
-          cp_async_commit();
-          cp_async_wait<0>();
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[e]);
+          page = next;
+          if ((e += 2) >= kRing) e -= kRing, ph ^= 1u;
         }
-        page = next;
-        if ((e += 2) >= kRing) e -= kRing, ph ^= 1u;
       }
       if (is_v) report();
       if (*abort_flag) {  // gave up: the copies in flight land before the CTA leaves
@@ -564,58 +813,65 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   }
 }
 
-// Joins the cache ranges of a row: a warp per (token, query head) adds up the ranges' unnormalised rows, each weighted by
-// 2^(its reference point - the largest one), and divides by the likewise weighted sum of their sums.
+// Joins the row tiles that were cut: the run that holds a tile's end (blockIdx.x) adds up the runs' unnormalised rows, a
+// warp per row, each part weighted by 2^(its reference point - the largest one), and divides by the likewise weighted
+// sum of their sums.
 template <bool kHalf, int kDim>
 __global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkArgs ka) {
-  __shared__ float qs[4][kDim];
   const subspec_chunk_attn_args& a = ka.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = ka.group;
-  const long long r = (long long)blockIdx.x * 4 + warp;
   grid_dep_wait();
-  if (r >= (long long)a.tokens * a.num_q_heads) return;
-  const int t = (int)(r / a.num_q_heads), head = (int)(r - (long long)t * a.num_q_heads);
-  const int b = request_of(a.q_indptr, a.batch, t);
-  if (b < 0) return;
-  const Request rq = read_request(a, b, false);
-  const int i = t - rq.q0;
-  if (i >= rq.n || rq.n * G <= ka.few_rows) return;
-  // the row tile this row was part of, its list of cache tiles, and how that was cut
-  const int row0 = (i * G + head % G) / kCtaRows * kCtaRows;
-  const TileList<kTileKeys> tiles(rq.first_pos + row0 / G, rq.first_pos + (min(row0 + kCtaRows, rq.n * G) - 1) / G, a.window, a.sinks);
-  const int per = per_split(tiles.n, ka.splits);
-  if (per >= tiles.n) return;  // one CTA did it all
-  const int parts = (tiles.n + per - 1) / per;
-  const float* ml = ka.part_ml + (size_t)r * ka.splits * 2;
-  float mstar = -INFINITY;
-  for (int s = 0; s < parts; ++s) mstar = ml[2 * s + 1] != 0.f ? max3_nan(mstar, ml[2 * s], ml[2 * s]) : mstar;
+  const int4 rec = ka.runs[blockIdx.x];
+  if (rec.w != 3) return;  // not the end of a row tile that began in an earlier run
+  const int c1 = (int)blockIdx.x;
+  int c0 = c1 - 1;
+  while (c0 > 0 && ka.runs[c0].w == 1) --c0;  // runs that lie inside the row tile
+  const Request rq = read_request(a, rec.x, false);
   constexpr int kPer = kDim / 32;
-  float acc[kPer] = {}, lsum = 0.f;
-  for (int s = 0; s < parts; ++s) {
-    const float l = ml[2 * s + 1];
-    if (l == 0.f) continue;  // nothing seen in this range
-    const float w = ex2f(ml[2 * s] - mstar);
-    const float* o = ka.part_o + ((size_t)r * ka.splits + s) * kDim + lane * kPer;
+  for (int r = (int)blockIdx.y * 4 + warp; r < kCtaRows; r += 4 * (int)gridDim.y) {
+    const int row = rec.z * kCtaRows + r;
+    if (row >= rq.n * G) return;
+    const int tok = row / G, head = rec.y * G + row - tok * G, t = rq.q0 + tok, pos = rq.first_pos + tok;
+    auto part = [&](int c) { return ((size_t)2 * c + (c == c0 ? 1 : 0)) * kCtaRows + r; };
+    float mstar = -INFINITY;
+    for (int c = c0 + lane; c <= c1; c += 32) {
+      const float2 ml = reinterpret_cast<const float2*>(ka.part_ml)[part(c)];
+      if (ml.y != 0.f) mstar = max3_nan(mstar, ml.x, ml.x);
+    }
 #pragma unroll
-    for (int c = 0; c < kPer; ++c) acc[c] += w * o[c];
-    lsum += w * l;
-  }
-  const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
-  bool odd = lsum == 0.f;
+    for (int d = 16; d; d >>= 1) {
+      const float y = __shfl_xor_sync(0xffffffffu, mstar, d);
+      mstar = max3_nan(mstar, y, y);
+    }
+    float acc[kPer] = {}, lsum = 0.f;
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      const float2 ml = reinterpret_cast<const float2*>(ka.part_ml)[part(c)];
+      float o[kPer];
 #pragma unroll
-  for (int c = 0; c < kPer; ++c) {
-    acc[c] *= inv;
-    odd = odd || !(fabsf(acc[c]) < INFINITY);
-  }
-  const int pos = rq.first_pos + i;
-  if (__any_sync(0xffffffffu, odd) && lsum == lsum && pos >= 0) {  // see the epilogue above
-    attn_row<kHalf, kDim>(ka, b, pos, t, head, qs[warp]);
-    return;
-  }
-  uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + (size_t)t * a.o_token_stride +
-                                              (size_t)head * a.o_head_stride);
+      for (int x = 0; x < kPer; ++x) o[x] = ka.part_o[part(c) * kDim + lane * kPer + x];
+      if (ml.y == 0.f) continue;  // nothing seen in this part
+      const float w = ex2f(ml.x - mstar);
 #pragma unroll
-  for (int c = 0; c < kPer / 2; ++c) out[lane * (kPer / 2) + c] = pack16<kHalf>(acc[2 * c], acc[2 * c + 1]);
+      for (int x = 0; x < kPer; ++x) acc[x] += w * o[x];
+      lsum += w * ml.y;
+    }
+    const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
+    bool odd = lsum == 0.f;
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) {
+      acc[c] *= inv;
+      odd = odd || !(fabsf(acc[c]) < INFINITY);
+    }
+    if (__any_sync(0xffffffffu, odd) && lsum == lsum && pos >= 0) {  // see the epilogue above
+      attn_row<kHalf, kDim>(ka, rec.x, pos, t, head);
+      continue;
+    }
+    uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + (size_t)t * a.o_token_stride +
+                                                (size_t)head * a.o_head_stride);
+#pragma unroll
+    for (int c = 0; c < kPer / 2; ++c) out[lane * (kPer / 2) + c] = pack16<kHalf>(acc[2 * c], acc[2 * c + 1]);
+  }
 }
 
 int check_args(const subspec_chunk_attn_args* args) {
@@ -623,7 +879,7 @@ int check_args(const subspec_chunk_attn_args* args) {
   const subspec_chunk_attn_args& a = *args;
   if (a.batch < 0 || a.tokens < 0 || a.max_q_len < 0 || a.num_q_heads < 1 || a.num_kv_heads < 1 || a.layers < 1 ||
       a.layer < 0 || a.layer >= a.layers || a.num_pages < 1 || a.page_len < 1 || a.pages_per_seq < 1 || a.window < 0 ||
-      a.sinks < 0 || a.kv_splits < 0 || a.kv_splits > 1024 || !(a.sm_scale > 0.0) ||
+      a.sinks < 0 || !(a.sm_scale > 0.0) ||
       (a.dtype != SUBSPEC_BF16 && a.dtype != SUBSPEC_F16))
     return SUBSPEC_EINVAL;
   if ((a.head_dim != 64 && a.head_dim != 128) || a.num_q_heads % a.num_kv_heads ||
@@ -647,35 +903,23 @@ static void chunk_sizes(ChunkArgs& ka) {
   const long long others = (long long)(a.tokens - a.max_q_len) * ka.group;
   ka.few_rows = most <= 16 ? 16 : most <= 32 ? 32 : a.batch > 1 && others <= 64LL * (a.batch - 1) ? 16 : 0;
   if (ka.few_rows >= most) {
-    ka.items = 0;
-    ka.splits = 1;
+    ka.ctas = 0;
     return;
   }
+  // A CTA per SM, or fewer where even the longest caches of the table's width make fewer runs.
   const long long by_tokens = (long long)a.tokens * ka.group / kCtaRows + a.batch;
   const long long by_batch = (long long)a.batch * ((most + kCtaRows - 1) / kCtaRows);
-  ka.items = (int)(by_tokens < by_batch ? by_tokens : by_batch);
-  // Few row tiles with long caches would leave SMs idle: as many ranges as fill them once, none shorter than
-  // kMinSplitTiles at the table's full width (shorter caches are cut into fewer ranges on the device).
-  const long long ctas = (long long)ka.items * a.num_kv_heads;
+  const long long row_tiles = (by_tokens < by_batch ? by_tokens : by_batch) * a.num_kv_heads;
   const long long cap = (long long)a.pages_per_seq * a.page_len;
-  const long long seen = a.window > 0 ? (long long)a.window + a.sinks + a.max_q_len : cap;
-  const long long tiles = ((seen < cap ? seen : cap) + kTileKeys - 1) / kTileKeys;
-  long long s = a.kv_splits;
-  if (s == 0) {
-    s = kNumSMs / (ctas > 0 ? ctas : 1);
-    if (s > tiles / kMinSplitTiles) s = tiles / kMinSplitTiles;
-    if (s > 32) s = 32;
-    if (s < 1) s = 1;
-  }
-  ka.splits = (int)s;
+  const long long seen = a.window > 0 ? (long long)a.window + a.sinks + a.max_q_len + 2 * kTileKeys : cap;
+  const long long runs = row_tiles * ((seen < cap ? seen : cap) / kTileKeys + 3) / kMinRun + 1;
+  ka.ctas = (int)(runs < kNumSMs ? runs : kNumSMs);
 }
 
-static size_t split_floats(const ChunkArgs& ka) {
-  if (ka.splits <= 1) return 0;
-  return (size_t)ka.a.tokens * ka.a.num_q_heads * ka.splits * (ka.a.head_dim + 2);
-}
+// Scratch: the runs' records (both kernels'), then the parts of the one, then those of the other.
+static size_t part_floats(const ChunkArgs& ka) { return (size_t)2 * ka.ctas * kCtaRows * (ka.a.head_dim + 2); }
 static size_t chunk_scratch_bytes(const ChunkArgs& ka) {
-  return (split_floats(ka) + (ka.few_rows ? chunk_few_floats(ka) : 0)) * sizeof(float);
+  return (size_t)ka.ctas * sizeof(int4) + part_floats(ka) * sizeof(float) + (ka.few_rows ? chunk_few_scratch_bytes(ka) : 0);
 }
 
 extern "C" int subspec_chunk_attention_scratch_bytes(const subspec_chunk_attn_args* args, size_t* bytes) {
@@ -720,19 +964,14 @@ void chunk_tensor_maps(ChunkArgs& ka, int rows, CUtensorMap* k, CUtensorMap* v) 
 
 template <bool kHalf, int kDim>
 static int launch_chunk(ChunkArgs& ka, cudaStream_t stream) {
-  const subspec_chunk_attn_args& a = ka.a;
   const int rc = allow_smem<chunk_attn_tc_kernel<kHalf, kDim>>(tc_smem<kDim>());
   if (rc) return rc;
   CUtensorMap tmap_k, tmap_v;
   chunk_tensor_maps(ka, kTileKeys, &tmap_k, &tmap_v);
-  chunk_attn_tc_kernel<kHalf, kDim><<<dim3((unsigned)(ka.items * ka.splits), (unsigned)a.num_kv_heads), kChunkThreads,
-                                      tc_smem<kDim>(), stream>>>(ka, tmap_k, tmap_v);
-  if (ka.splits > 1) {
-    const long long rows = (long long)a.tokens * a.num_q_heads;
-    const int rc2 = cuda_check(cudaGetLastError());
-    return rc2 ? rc2 : launch_dependent(chunk_merge_kernel<kHalf, kDim>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, ka);
-  }
-  return cuda_check(cudaGetLastError());
+  chunk_attn_tc_kernel<kHalf, kDim><<<ka.ctas, kChunkThreads, tc_smem<kDim>(), stream>>>(ka, tmap_k, tmap_v);
+  const int launched = cuda_check(cudaGetLastError());
+  if (launched) return launched;
+  return launch_dependent(chunk_merge_kernel<kHalf, kDim>, dim3((unsigned)ka.ctas, 16), dim3(128), 0, stream, ka);
 }
 
 extern "C" int subspec_chunk_attention_paged(const subspec_chunk_attn_args* args, subspec_stream_t stream) {
@@ -762,12 +1001,13 @@ extern "C" int subspec_chunk_attention_paged(const subspec_chunk_attn_args* args
   ka.units = (int)units;
   const size_t need = chunk_scratch_bytes(ka);
   if (need && (!a.scratch || (reinterpret_cast<uintptr_t>(a.scratch) & 15u) || a.scratch_bytes < need)) return SUBSPEC_ESCRATCH;
-  ka.part_o = reinterpret_cast<float*>(a.scratch);
-  ka.part_ml = ka.part_o + (size_t)a.tokens * a.num_q_heads * ka.splits * a.head_dim;
+  ka.runs = reinterpret_cast<int4*>(a.scratch);
+  ka.part_o = reinterpret_cast<float*>(ka.runs + ka.ctas);
+  ka.part_ml = ka.part_o + (size_t)2 * ka.ctas * kCtaRows * a.head_dim;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (ka.few_rows) {
-    rc = launch_chunk_few(ka, ka.part_o + split_floats(ka), st);
-    if (rc || ka.items == 0) return rc;
+    rc = launch_chunk_few(ka, ka.part_o + part_floats(ka), st);
+    if (rc || ka.ctas == 0) return rc;
   }
   if (a.dtype == SUBSPEC_F16) return a.head_dim == 128 ? launch_chunk<true, 128>(ka, st) : launch_chunk<true, 64>(ka, st);
   return a.head_dim == 128 ? launch_chunk<false, 128>(ka, st) : launch_chunk<false, 64>(ka, st);

@@ -20,30 +20,17 @@ struct ChunkArgs {
   const unsigned char* v_base;
   long long page_stride, row_stride;
   int page_units, units;  // a page, and the whole layer, in rows of one head (the tensor maps' outermost coordinate)
-  int items;              // row tiles the grid has room for, per KV head
-  int splits;             // CTAs that may share a row tile's cache tiles
-  float* part_o;          // splits > 1: [token][head][split][head_dim] unnormalised outputs
-  float* part_ml;         //             [token][head][split][2] reference point (log2 units) and sum
+  int ctas;               // of the kernel for many rows (0: not launched)
+  int4* runs;             // its runs: request, KV head, row tile of the first piece; 1: begun in an earlier run, 2: ends in this
+  float* part_o;          // [run][2][256][head_dim] unnormalised rows: [0] of a row tile begun earlier, [1] of one that goes on
+  float* part_ml;         // [run][2][256][2] reference point (log2 units) and sum
   int few_rows;           // requests of at most so many rows go to the kernel for few rows (0: none)
-  float* few_o;           // [part][few_rows][head_dim], [part][few_rows][2]: the same for its parts
+  int4* few_runs;         // the same for it
+  float* few_o;
   float* few_ml;
 };
 
 constexpr float kRescaleAt = 8.f;  // log2 units the maximum may run ahead of the exponents' reference point
-
-// The request of packed token t: the last b with q_indptr[b] <= t; -1 behind the last request.
-__device__ __forceinline__ int request_of(const int* q_indptr, int batch, int t) {
-  if (t < q_indptr[0] || t >= q_indptr[batch]) return -1;
-  int lo = 0, hi = batch - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (q_indptr[mid] <= t)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  return lo;
-}
 
 template <bool kHalf>
 __device__ __forceinline__ float2 unpack16(uint32_t w) {
@@ -51,17 +38,22 @@ __device__ __forceinline__ float2 unpack16(uint32_t w) {
   return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
 }
 
-// One row by a warp, key by key, touching nothing but the rows that it sees: a lane takes every 32nd row for the
-// scores, then every lane two (head_dim 64) or four dims of the output.  `qs`: head_dim floats of shared memory.
+// One row by a warp, key by key, touching nothing but the rows that it sees: every lane has two (head_dim 64) or four of
+// the dims, four keys at a time.  (What the tiles leave undone: see their epilogues.)
 template <bool kHalf, int kDim>
-__device__ void attn_row(const ChunkArgs& ka, int b, int pos, int t, int head, float* qs) {
+__device__ void attn_row(const ChunkArgs& ka, int b, int pos, int t, int head) {
   const subspec_chunk_attn_args& a = ka.a;
-  constexpr int kPer = kDim / 32;
+  constexpr int kPer = kDim / 32, kAtOnce = 4;
   const int lane = threadIdx.x & 31;
-  const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (size_t)t * a.q_token_stride + (size_t)head * a.q_head_stride;
-  __syncwarp();
-  for (int d = lane; d < kDim; d += 32) qs[d] = unpack16<kHalf>((uint32_t)q[d]).x * ka.scale_log2;
-  __syncwarp();
+  auto load = [&](const uint16_t* p, float (&x)[kPer]) {
+#pragma unroll
+    for (int c = 0; c < kPer / 2; ++c) {
+      const float2 y = unpack16<kHalf>(reinterpret_cast<const uint32_t*>(p)[lane * (kPer / 2) + c]);
+      x[2 * c] = y.x, x[2 * c + 1] = y.y;
+    }
+  };
+  float q[kPer];
+  load(reinterpret_cast<const uint16_t*>(a.q) + (size_t)t * a.q_token_stride + (size_t)head * a.q_head_stride, q);
   const size_t row = (size_t)a.num_kv_heads * kDim, plane = (size_t)a.page_len * row;
   const uint16_t* pool = reinterpret_cast<const uint16_t*>(a.pool) + (size_t)a.layer * a.num_pages * 2 * plane +
                          (size_t)(head / ka.group) * kDim;
@@ -70,56 +62,49 @@ __device__ void attn_row(const ChunkArgs& ka, int b, int pos, int t, int head, f
   const int head_rows = min(a.window > 0 ? a.sinks : 0, lo);  // rows [0, head_rows) and [lo, pos]
   const int seen = head_rows + pos + 1 - lo;
   float m = -INFINITY, l = 0.f, o[kPer] = {};
-  for (int j0 = 0; j0 < seen; j0 += 32) {
-    const int idx = j0 + lane, j = idx < head_rows ? idx : lo + idx - head_rows;
-    long long at = -1;  // element offset of the K row
-    float s = -INFINITY;
-    if (idx < seen) {
+  for (int j0 = 0; j0 < seen; j0 += kAtOnce) {
+    float s[kAtOnce], v[kAtOnce][kPer];
+#pragma unroll
+    for (int x = 0; x < kAtOnce; ++x) {
+      const int idx = j0 + x, j = idx < head_rows ? idx : lo + idx - head_rows;
+      s[x] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) v[x][c] = 0.f;
+      if (idx >= seen) continue;
       const int pi = j / a.page_len, pg = table[pi];
-      if (pg >= 0 && pg < a.num_pages) {
-        at = (long long)((size_t)pg * 2 * plane + (size_t)(j - pi * a.page_len) * row);
-        const uint4* k = reinterpret_cast<const uint4*>(pool + at);
-        s = 0.f;
-#pragma unroll 4
-        for (int c = 0; c < kDim / 8; ++c) {
-          const uint4 w = k[c];
-          const float2 x0 = unpack16<kHalf>(w.x), x1 = unpack16<kHalf>(w.y), x2 = unpack16<kHalf>(w.z), x3 = unpack16<kHalf>(w.w);
-          const float* p = qs + 8 * c;
-          s += p[0] * x0.x + p[1] * x0.y + p[2] * x1.x + p[3] * x1.y + p[4] * x2.x + p[5] * x2.y + p[6] * x3.x + p[7] * x3.y;
-        }
-      } else {
+      if (pg < 0 || pg >= a.num_pages) {
         flag(a.dev_status, SUBSPEC_DEV_BAD_PAGE);
-        s = 0.f;  // a row of zeros, as the tiles hold it
+        continue;  // a row of zeros, as the tiles hold it
       }
-    }
-    float mx = s;
+      const uint16_t* at = pool + (size_t)pg * 2 * plane + (size_t)(j - pi * a.page_len) * row;
+      float k[kPer];
+      load(at, k);
+      load(at + plane, v[x]);
 #pragma unroll
-    for (int d = 16; d; d >>= 1) {
-      const float y = __shfl_xor_sync(0xffffffffu, mx, d);
-      mx = (mx != mx || y != y) ? NAN : fmaxf(mx, y);
+      for (int c = 0; c < kPer; ++c) s[x] += q[c] * k[c];
     }
-    mx = (m != m) ? m : ((mx != mx) ? mx : fmaxf(m, mx));
-    const float old = (m == -INFINITY) ? 0.f : exp2f(m - mx);  // nothing summed yet: nothing to rescale
-    const float p = idx < seen && mx != -INFINITY ? exp2f(s - mx) : 0.f;  // (scores of -inf so far: weight 0)
-    float ps = p;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, d);
-    l = l * old + ps;
+    for (int d = 16; d; d >>= 1)
+#pragma unroll
+      for (int x = 0; x < kAtOnce; ++x) s[x] += __shfl_xor_sync(0xffffffffu, s[x], d);
+    float mx = m;
+#pragma unroll
+    for (int x = 0; x < kAtOnce; ++x) {
+      s[x] = j0 + x < seen ? s[x] * ka.scale_log2 : -INFINITY;
+      mx = (mx != mx || s[x] != s[x]) ? NAN : fmaxf(mx, s[x]);
+    }
+    const float old = m == -INFINITY ? 0.f : exp2f(m - mx);  // nothing summed yet: nothing to rescale
     m = mx;
+    l *= old;
 #pragma unroll
     for (int c = 0; c < kPer; ++c) o[c] *= old;
-    const int n = min(32, seen - j0);
-    for (int i = 0; i < n; ++i) {
-      const float w = __shfl_sync(0xffffffffu, p, i);
-      const long long ra = __shfl_sync(0xffffffffu, at, i);
-      if (ra < 0) continue;
-      const uint32_t* v = reinterpret_cast<const uint32_t*>(pool + ra + plane);
 #pragma unroll
-      for (int c = 0; c < kPer / 2; ++c) {
-        const float2 x = unpack16<kHalf>(v[lane * (kPer / 2) + c]);
-        o[2 * c] += w * x.x;
-        o[2 * c + 1] += w * x.y;
-      }
+    for (int x = 0; x < kAtOnce; ++x) {
+      if (j0 + x >= seen) continue;
+      const float p = mx == -INFINITY ? 0.f : exp2f(s[x] - mx);  // (scores of -inf so far: weight 0)
+      l += p;
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) o[c] += p * v[x][c];
     }
   }
   const float inv = seen > 0 ? 1.f / l : 0.f;
@@ -134,6 +119,7 @@ __device__ void attn_row(const ChunkArgs& ka, int b, int pos, int t, int head, f
 // those from the lowest window row to the highest token.
 template <int kTile>
 struct TileList {
+  TileList() = default;
   int hi, lo, snk;  // rows [0, snk) and [lo, hi)
   int s_tiles, m0, n;
   __device__ __forceinline__ TileList(int pmin, int pmax, int window, int sinks) {
@@ -179,6 +165,11 @@ __device__ __forceinline__ Request read_request(const subspec_chunk_attn_args& a
   if (r.q0 < 0 || q1 > a.tokens || q1 < r.q0) r.n = 0;
   if (report && (r.n != n || q1 < r.q0 || kv < n || kv > cap)) flag(a.dev_status, SUBSPEC_DEV_BAD_COUNT);
   return r;
+}
+
+__device__ __forceinline__ Request shfl_request(const Request& r, int src) {
+  return Request{__shfl_sync(0xffffffffu, r.q0, src), __shfl_sync(0xffffffffu, r.n, src), __shfl_sync(0xffffffffu, r.first_pos, src),
+                 __shfl_sync(0xffffffffu, r.kv_len, src)};
 }
 
 }  // namespace subspec

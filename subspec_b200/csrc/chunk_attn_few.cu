@@ -93,7 +93,6 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   constexpr int kSteps = kDim / 16;
   __shared__ __align__(8) uint64_t full[kFewWarps][kStages];
   __shared__ float s_ml[kFewWarps][16][2];
-  __shared__ float s_q[kFewWarps][kDim];
   __shared__ int s_abort;
   const subspec_chunk_attn_args& a = ka.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = ka.group, H = a.num_kv_heads;
@@ -112,7 +111,10 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   }
   total *= H;
   const int runs = few_runs(total, (int)gridDim.x), run = (int)blockIdx.x;
-  if (total == 0 || run >= runs) return;
+  if (total == 0 || run >= runs) {
+    if (threadIdx.x == 0) ka.few_runs[run] = make_int4(0, 0, 0, 0);
+    return;
+  }
   const long long g0 = run * total / runs, g1 = (run + 1) * total / runs;
   Cursor at;
   {
@@ -141,6 +143,10 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     at.h = (int)(rem / at.n);
     at.i = (int)(rem - (long long)at.h * at.n);
   }
+
+  // what the join needs: the run's first (request, head), whether it began in an earlier run, whether it ends in this one
+  if (threadIdx.x == 0)
+    ka.few_runs[run] = make_int4(at.b, at.h, 0, (at.i > 0 ? 1 : 0) | (at.i + (g1 - g0) >= at.n ? 2 : 0));
 
   unsigned char* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u) + (size_t)warp * kStages * kStageBytes;
   const int box = ka.box_rows, boxes = box > 0 ? kWarpKeys / box : 0;
@@ -422,7 +428,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
         const int src = __ffs(again) - 1;
         again &= ~(0xffu << (src & ~7));  // the eight lanes of a row
         attn_row<kHalf, kDim>(ka, at.b, __shfl_sync(0xffffffffu, row_pos, src), __shfl_sync(0xffffffffu, t, src),
-                              __shfl_sync(0xffffffffu, head, src), s_q[warp]);
+                              __shfl_sync(0xffffffffu, head, src));
       }
       __syncthreads();
     }
@@ -440,46 +446,22 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   }
 }
 
-// Joins the parts of a (request, KV head) that lies in several runs: a CTA per (token, query head).
+// Joins the (request, KV head)s that lie in several runs: a CTA per (run that holds the end of one, row).
 template <bool kHalf, int kDim, int kMT>
-__global__ void __launch_bounds__(128) chunk_few_join_kernel(const ChunkArgs ka, int ctas) {
-  __shared__ long long s_sum[2][4];
+__global__ void __launch_bounds__(128) chunk_few_join_kernel(const ChunkArgs ka) {
   __shared__ float s_acc[128][9];
-  __shared__ float s_q[kDim];
   const subspec_chunk_attn_args& a = ka.a;
-  const int t = (int)(blockIdx.x / a.num_q_heads), head = (int)(blockIdx.x % a.num_q_heads);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = ka.group, H = a.num_kv_heads;
-  // (the lengths were there before the kernel in front began)
-  const int b = request_of(a.q_indptr, a.batch, t);
-  const Request rq = read_request(a, max(b, 0), false);
-  const int tiles = few_tiles(ka, rq, nullptr), i = t - rq.q0;
-  if (b < 0 || tiles == 0 || i >= rq.n) {
-    grid_dep_wait();
-    return;
-  }
-  // tiles in front of the request, and all of them
-  long long before = 0, total = 0;
-  for (int x = (int)threadIdx.x; x < a.batch; x += 128) {
-    const int n = few_tiles(ka, read_request(a, x, false), nullptr);
-    total += n;
-    if (x < b) before += n;
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, d);
-    total += __shfl_xor_sync(0xffffffffu, total, d);
-  }
-  if (lane == 0) s_sum[0][warp] = before, s_sum[1][warp] = total;
-  __syncthreads();
-  before = H * (s_sum[0][0] + s_sum[0][1] + s_sum[0][2] + s_sum[0][3]);
-  total = H * (s_sum[1][0] + s_sum[1][1] + s_sum[1][2] + s_sum[1][3]);
-  const int runs = few_runs(total, ctas);
-  const long long s0 = before + (long long)(head / G) * tiles, s1 = s0 + tiles;
-  // the run that holds tile x: the largest c with floor(c total / runs) <= x
-  const int c0 = (int)(((s0 + 1) * runs - 1) / total), c1 = (int)((s1 * runs - 1) / total);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = ka.group, grow = (int)blockIdx.y;
   grid_dep_wait();
-  if (c0 == c1) return;  // written by the run itself
-  const int grow = i * G + head % G;
+  const int4 rec = ka.few_runs[blockIdx.x];
+  if (rec.w != 3) return;
+  const int c1 = (int)blockIdx.x;
+  int c0 = c1 - 1;
+  while (c0 > 0 && ka.few_runs[c0].w == 1) --c0;  // runs that lie inside it
+  const int b = rec.x;
+  const Request rq = read_request(a, b, false);
+  const int i = grow / G, t = rq.q0 + i, head = rec.y * G + grow - i * G;
+  if (i >= rq.n) return;
   constexpr int kChunks = kDim / 8, kGroups = 128 / kChunks;
   const int ch = (int)threadIdx.x % kChunks, grp = (int)threadIdx.x / kChunks;
   auto row_of = [&](int c) { return ((size_t)2 * c + (c == c0 ? 1 : 0)) * (16 * kMT) + grow; };
@@ -534,7 +516,7 @@ __global__ void __launch_bounds__(128) chunk_few_join_kernel(const ChunkArgs ka,
                                pack16<kHalf>(acc[6], acc[7]));
     reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + (size_t)t * a.o_token_stride + (size_t)head * a.o_head_stride)[lane] = v;
   }
-  if (__any_sync(0xffffffffu, odd)) attn_row<kHalf, kDim>(ka, b, pos, t, head, s_q);
+  if (__any_sync(0xffffffffu, odd)) attn_row<kHalf, kDim>(ka, b, pos, t, head);
 }
 
 template <bool kHalf, int kDim, int kMT>
@@ -546,8 +528,9 @@ int launch(ChunkArgs& ka, cudaStream_t stream) {
   chunk_attn_few_kernel<kHalf, kDim, kMT><<<kFewCtas, kFewThreads, few_smem<kDim>(), stream>>>(ka, tmap_k, tmap_v);
   const int launched = cuda_check(cudaGetLastError());
   if (launched) return launched;
-  const long long rows = (long long)ka.a.tokens * ka.a.num_q_heads;
-  return launch_dependent(chunk_few_join_kernel<kHalf, kDim, kMT>, dim3((unsigned)rows), dim3(128), 0, stream, ka, kFewCtas);
+  const long long rows = (long long)ka.a.max_q_len * ka.group;
+  return launch_dependent(chunk_few_join_kernel<kHalf, kDim, kMT>, dim3(kFewCtas, (unsigned)(rows < 16 * kMT ? rows : 16 * kMT)),
+                          dim3(128), 0, stream, ka);
 }
 
 template <int kMT>
@@ -558,11 +541,14 @@ int launch_mt(ChunkArgs& ka, cudaStream_t stream) {
 
 }  // namespace
 
-size_t chunk_few_floats(const ChunkArgs& ka) { return (size_t)2 * kFewCtas * ka.few_rows * (ka.a.head_dim + 2); }
+size_t chunk_few_scratch_bytes(const ChunkArgs& ka) {
+  return kFewCtas * sizeof(int4) + (size_t)2 * kFewCtas * ka.few_rows * (ka.a.head_dim + 2) * sizeof(float);
+}
 
 int launch_chunk_few(ChunkArgs& ka, float* scratch, cudaStream_t stream) {
-  ka.few_o = scratch;
-  ka.few_ml = scratch + (size_t)2 * kFewCtas * ka.few_rows * ka.a.head_dim;
+  ka.few_runs = reinterpret_cast<int4*>(scratch);
+  ka.few_o = reinterpret_cast<float*>(ka.few_runs + kFewCtas);
+  ka.few_ml = ka.few_o + (size_t)2 * kFewCtas * ka.few_rows * ka.a.head_dim;
   return ka.few_rows == 16 ? launch_mt<1>(ka, stream) : launch_mt<2>(ka, stream);
 }
 

@@ -257,14 +257,26 @@ def test_page_lengths(cuda_lib, page_len):
     _run_and_check(c, 50, 3, max_q_len=2)
 
 
-@pytest.mark.parametrize("splits", [1, 2, 5, 16])
-def test_cache_ranges(cuda_lib, splits):
-    """The same rows with the cache cut into ranges for several CTAs; more ranges than tiles among them."""
-    for new, cached in (([1, 1, 1], [900, 40, 0]), ([60, 3], [700, 90])):
-        c = _setup(5, new, cached, 14, 2)
-        _run_and_check(c, kv_splits=splits)
-        _run_and_check(c, 130, 5, kv_splits=splits)
-        _run_and_check(c, kv_splits=splits, max_q_len=max(new))
+@pytest.mark.parametrize("new,cached", [
+    ([1], [9000]), ([1, 1, 1], [3000, 40, 0]), ([3], [5000]), ([60, 3], [2700, 90]), ([300], [4000]), ([9, 1, 200], [64, 3000, 1500])])
+@pytest.mark.parametrize("heads,kv_heads", [(14, 2), (4, 1)])
+def test_caches_cut_into_runs(cuda_lib, new, cached, heads, kv_heads):
+    """Few requests behind long caches: their cache rows are shared between many CTAs and joined."""
+    c = _setup(5, new, cached, heads, kv_heads)
+    _run_and_check(c)
+    _run_and_check(c, 1300, 5)
+    _run_and_check(c, max_q_len=max(new))
+
+
+def test_many_requests(cuda_lib):
+    """More requests than a warp has lanes and than are summed side by side; ones that bring nothing among them."""
+    new = [[0, 1, 2, 7, 40, 0, 1, 19][i % 8] for i in range(150)]
+    cached = [(37 * i) % 300 for i in range(150)]
+    c = _setup(19, new, cached, 4, 1, D=64)
+    _run_and_check(c)
+    _run_and_check(c, 60, 3)
+    c = _setup(20, [min(n, 1) for n in new], cached, 8, 1)
+    _run_and_check(c, max_q_len=1)
 
 
 WINDOWS = [(1, 0), (1, 1), (2, 300), (16, 0), (100, 4), (128, 128), (129, 130), (5000, 7)]
@@ -288,7 +300,7 @@ def test_pages_behind_the_window_may_be_gone(cuda_lib):
             if j * 16 >= sinks and (j + 1) * 16 <= first:
                 c["table"][0, j] = -1
         _run_and_check(c, window, sinks)
-        _run_and_check(c, window, sinks, max_q_len=new[0], kv_splits=3)
+        _run_and_check(c, window, sinks, max_q_len=new[0])
 
 
 @pytest.mark.parametrize("new", [[1, 1], [3, 2], [90, 40], [300, 1]])
@@ -315,7 +327,7 @@ def test_hidden_rows_have_no_influence(cuda_lib, new, bad):
         for j in range(10, 100):
             c["vs"][b][j] = c["ks"][b][j] = bad
             c["pool"][1, c["table"][b, j // 16], :, j % 16] = bad
-    for kw in (dict(), dict(max_q_len=max(new)), dict(kv_splits=2)):
+    for kw in (dict(), dict(max_q_len=max(new)), dict(max_q_len=512)):
         got = _run(c, 50, 10, **kw).float().cpu()
         for b, n in enumerate(new):
             lo, first = c["indptr"][b], [200, 150][b]
@@ -415,7 +427,7 @@ def test_random_shapes(cuda_lib, seed):
     c = _setup(900 + seed, new, cached, heads, kv_heads, D=[64, 128][r(0, 1)], page_len=[1, 8, 16, 16, 20, 32, 64, 256][r(0, 7)],
                dtype=[torch.bfloat16, torch.float16][r(0, 1)])
     window = [0, 0, r(1, 900)][r(0, 2)]
-    _run_and_check(c, window, r(0, 40) if window else 0, max_q_len=[None, most][r(0, 1)], kv_splits=[None, None, r(1, 9)][r(0, 2)])
+    _run_and_check(c, window, r(0, 40) if window else 0, max_q_len=[None, most][r(0, 1)])
 
 
 def test_results_do_not_depend_on_the_run(cuda_lib):

@@ -41,7 +41,7 @@ def _call(fn=chunk_attention_paged, **kw):
     dict(q_indptr=_i32(0, 2)), dict(q_indptr=torch.tensor([0, 2, 3])),
     dict(out=torch.zeros(3, 4, 64)), dict(out=torch.zeros(2, 4, 64, dtype=torch.bfloat16)),
     dict(out=torch.zeros(3, 4, 65, dtype=torch.bfloat16)[..., 1:]),          # rows not 16-byte aligned
-    dict(kv_splits=0), dict(kv_splits=2000), dict(max_q_len=-1),
+    dict(max_q_len=-1),
 ])
 def test_attention_refusals(bad):
     with pytest.raises(ValueError):
@@ -114,7 +114,7 @@ def test_c_entry_points_check_their_arguments(cuda_lib):
     assert cuda_lib.subspec_chunk_attention_scratch_bytes(C.byref(a), C.byref(n)) == _lib.OK
     for name, bad, rc in (("sm_scale", 0.0, _lib.EINVAL), ("sm_scale", float("nan"), _lib.EINVAL), ("dtype", 7, _lib.EINVAL),
                           ("window", -1, _lib.EINVAL), ("sinks", -1, _lib.EINVAL), ("layer", 1, _lib.EINVAL),
-                          ("kv_splits", 5000, _lib.EINVAL), ("head_dim", 80, _lib.EUNSUPPORTED),
+                          ("head_dim", 80, _lib.EUNSUPPORTED),
                           ("num_q_heads", 3, _lib.EUNSUPPORTED)):
         old = getattr(a, name)
         setattr(a, name, bad)
