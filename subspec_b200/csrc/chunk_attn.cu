@@ -35,12 +35,12 @@ namespace {
 //               summing P in fp32.  m, the reference point, is the maximum of the first tile, and moves (the row of O in
 //               tensor memory is rescaled) only when the sums say that a later score has run far ahead of it.  They also
 //               bring the row's Q.
-//   warp 8      issues the MMAs, one block after the other: O += P V (P from tensor memory, V MN-major as the cache has
+//   warps 8, 9  issue the MMAs of a block each, in turns: O += P V (P from tensor memory, V MN-major as the cache has
 //               it), in two halves of 64 cache rows as their P comes, then S = Q K^T of the next tile (128 x 128 x
 //               head_dim, both K-major in shared memory) over the P just consumed: the MMAs of a thread run in order.
 //               While one block is in its softmax the other's MMAs run.
-//   warp 9      walks the run and hands out its pieces.
-//   warp 10     brings the K tiles, warp 11 the V tiles, into a ring of five entries, K(0), V(0), K(1), V(1), ...
+//   warp 10     brings the K tiles, warp 11 the V tiles, into a ring of five entries, K(0), V(0), K(1), V(1), ...;
+//               warp 10 also walks the run and hands out its pieces.
 //
 // A tile lies in shared memory as 16 groups of 8 rows; a group as one (head_dim 64) or two halves of 64 dims, a half as
 // 8 rows of 128 bytes under the 128-byte swizzle: the layout the tensor cores read either way round, in which the rows
@@ -53,10 +53,10 @@ constexpr int kBlockRows = 128;
 constexpr int kCtaRows = 2 * kBlockRows;
 constexpr int kRing = 5;
 constexpr int kChunkThreads = 384;
-constexpr int kIssuerWarp = 8, kPieceWarp = 9, kLoadWarp = 10;
+constexpr int kIssuerWarp = 8, kLoadWarp = 10;
 constexpr uint32_t kBlockCols = 256, kOCol = 128;
 #ifndef KFMA
-#define KFMA 4
+#define KFMA 8
 #endif
 constexpr int kFmaEvery = KFMA;
 constexpr int kMinRun = 4;    // cost a run holds at least (its cache tiles and one for each row tile)
@@ -190,7 +190,7 @@ __device__ Place locate(const ChunkArgs& ka, long long g, const long long* group
   return at;
 }
 
-// A piece: what a run has of one row tile.  Warp 9 walks the run and hands the pieces to the other warps through shared
+// A piece: what a run has of one row tile.  Warp 10 walks the run and hands the pieces to the other warps through shared
 // memory (a walker of thirty words in every warp pushes the softmax's scores out of the registers).
 struct Piece {
   int valid;                    // 0: the run is over
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     chunk_attn_tc_kernel(const ChunkArgs ka, const __grid_constant__ CUtensorMap tmap_k,
                          const __grid_constant__ CUtensorMap tmap_v) {
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t full[kRing], empty[kRing], s_ready[2], p_ready[2][2], h_done[2], o_done[2], q_ready, fix, drained, pc_full[kPieces], pc_empty[kPieces];
+  __shared__ __align__(8) uint64_t full[kRing], empty[kRing], s_ready[2], p_ready[2][2], h_done[2], o_done[2], my_turn[2], q_ready, fix, drained[2], pc_full[kPieces], pc_empty[kPieces];
   __shared__ long long s_cost[kGroups];
   __shared__ Place s_place[2];
   __shared__ Piece s_piece[kPieces];
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kRing; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], 2);  // both blocks' issuers let go of an entry
     }
     for (int k = 0; k < 2; ++k) {
       mbar_init(&s_ready[k], 1);
@@ -289,6 +289,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       mbar_init(&p_ready[k][1], 4);
       mbar_init(&h_done[k], 1);
       mbar_init(&o_done[k], 1);
+      mbar_init(&my_turn[k], 1);
+      mbar_init(&drained[k], 1);
     }
     mbar_init(&q_ready, 8);
     for (int k = 0; k < kPieces; ++k) {
@@ -296,7 +298,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       mbar_init(&pc_empty[k], kPieceReaders);
     }
     mbar_init(&fix, 1);
-    mbar_init(&drained, 1);
     mbar_init_fence();
     s_abort = 0;
   }
@@ -354,7 +355,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 
   if (warp < 8) {
     // ================= softmax =================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int blk = warp >> 2, rr = (int)threadIdx.x & 127;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)blk * kBlockCols;
     const uint32_t o_addr = lane_base + kOCol;
@@ -406,57 +406,46 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         live = __all_sync(0xffffffffu, tc_wait(&s_ready[blk], seen & 1u, abort_flag));
         if (!live) break;
         tc_fence_after();
-        uint32_t r[4][32];
+        // Half a tile (64 scores) at a time in registers: all 128 would fill them and leave the compiler nothing to
+        // reorder with.  The second half's scores stay in tensor memory until the first half's P is done.
+        uint32_t r[2][32];
         tmem_ld32_async(lane_base, r[0]);
         tmem_ld32_async(lane_base + 32, r[1]);
-        tmem_wait_ld_dep(r[0]);
-        tmem_wait_ld_dep(r[1]);
-        tmem_ld32_async(lane_base + 64, r[2]);
-        tmem_ld32_async(lane_base + 96, r[3]);
         const bool masked = !block_sees_all(bfirst, blast, t0);
-        auto hide = [&](int c) {
+        auto hide = [&](uint32_t (&x)[32], int c) {
           const int p0 = t0 + 32 * c;
           uint32_t bits = bits_below(pos + 1 - p0);
           if (a.window > 0) bits &= ~bits_below(pos - a.window + 1 - p0) | bits_below(a.sinks - p0);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) r[c][j] = (bits >> j) & 1u ? r[c][j] : 0xff800000u;
+          for (int j = 0; j < 32; ++j) x[j] = (bits >> j) & 1u ? x[j] : 0xff800000u;
         };
-        auto max32 = [&](int c) {  // NaN stays NaN: a NaN score makes the row NaN
-          float mx[2] = {__uint_as_float(r[c][0]), __uint_as_float(r[c][1])};
-#pragma unroll
-          for (int j = 2; j < 30; j += 4) {
-            mx[0] = max3_nan(mx[0], __uint_as_float(r[c][j]), __uint_as_float(r[c][j + 1]));
-            mx[1] = max3_nan(mx[1], __uint_as_float(r[c][j + 2]), __uint_as_float(r[c][j + 3]));
-          }
-          mx[0] = max3_nan(mx[0], __uint_as_float(r[c][30]), __uint_as_float(r[c][31]));
-          return max3_nan(mx[0], mx[1], mx[1]) * c2;  // c2 > 0
-        };
-        // Weights need a reference point near the row's maximum, not the maximum itself: a tile is first tried against the
-        // old one, without looking for its maximum.  Every weight is positive, so a sum within kSumLimit proves that none
-        // is too large (for the 16-bit type and the fp32 sums); anything else (a larger sum, an overflow, NaN, a row that
-        // has seen nothing yet) moves the reference point to the maximum, rescales O and does the half tile again.
-        bool rest = false;  // the second half of the scores has arrived
-        auto arrive_rest = [&]() {
-          if (rest) return;
-          rest = true;
-          tmem_wait_ld_dep(r[2]);
-          tmem_wait_ld_dep(r[3]);
-          if (masked) hide(2), hide(3);
-        };
-        if (masked) hide(0), hide(1);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          if (half == 1) arrive_rest();
+          tmem_wait_ld_dep(r[0]);
+          tmem_wait_ld_dep(r[1]);
+          if (masked) hide(r[0], 2 * half), hide(r[1], 2 * half + 1);
+          // Weights need a reference point near the row's maximum, not the maximum itself: a tile is first tried against
+          // the old one, without looking for its maximum.  Every weight is positive, so a sum within kSumLimit proves that
+          // none is too large (for the 16-bit type and the fp32 sums); anything else (a larger sum, an overflow, NaN, a row
+          // that has seen nothing yet) moves the reference point to the maximum of the scores not yet handed over, rescales
+          // O and does the half tile again.
           bool move = half == 0 && m == -INFINITY, moved = false;
           uint32_t pk[2][16];
           float sum;
           for (;;) {
             if (__any_sync(0xffffffffu, move)) {
               moved = true;
-              float alpha = 1.f;
-              arrive_rest();
-              float top = max3_nan(max32(2), max32(3), m);
-              if (half == 0) top = max3_nan(max32(0), max32(1), top);
+              float top = m, alpha = 1.f;
+              for (int c = 2 * half; c < 4; ++c) {  // NaN stays NaN: a NaN score makes the row NaN
+                uint32_t x[32];
+                tmem_ld32_async(lane_base + 32 * c, x);
+                tmem_wait_ld_dep(x);
+                if (masked) hide(x, c);
+                float mx = __uint_as_float(x[0]);
+#pragma unroll
+                for (int j = 1; j < 31; j += 2) mx = max3_nan(mx, __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
+                top = max3_nan(top, max3_nan(mx, __uint_as_float(x[31]), mx) * c2, top);  // c2 > 0
+              }
               if (move) {
                 alpha = m == -INFINITY ? 0.f : ex2f(m - top);
                 m = top;
@@ -466,7 +455,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 tc_fence_after();
               }
               if ((done > 0 || half == 1) && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < kDim / 32; ++c) {
                   uint32_t rc[32];
                   tmem_ld32_async(o_addr + 32 * c, rc);
@@ -485,9 +474,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             for (int c = 0; c < 2; ++c) {
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
-                const uint32_t* s = &r[2 * half + c][2 * j];
                 float x0, x1, p0, p1;
-                f2_unpack(f2_fma(f2_pack(__uint_as_float(s[0]), __uint_as_float(s[1])), c2p, nup), x0, x1);
+                f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c][2 * j]), __uint_as_float(r[c][2 * j + 1])), c2p, nup), x0, x1);
                 if (j % kFmaEvery == kFmaEvery - 1) {
                   exp2_pair(x0, x1, p0, p1);  // some pairs on the FMA pipe
                 } else {
@@ -503,6 +491,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             sum = e0 + e1;
             move = !(sum <= kSumLimit);
             if (moved || !__any_sync(0xffffffffu, move)) break;
+          }
+          if (half == 0) {
+            tmem_ld32_async(lane_base + 64, r[0]);
+            tmem_ld32_async(lane_base + 96, r[1]);
           }
           l += sum;
           tmem_st16(lane_base + 32 * half, pk[0]);
@@ -579,70 +571,76 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    if (warp == kIssuerWarp) {
-      // ================= MMA issue: one warp for both blocks, an elected lane issues =================
-      // One issuer, one block after the other: with an issuer per block the two blocks' MMAs interleave, both get
-      // their scores at the same time and then both sit in their softmax while the tensor cores idle (4660 cycles a
-      // tile against 2048 of MMAs).
+    if (warp < kLoadWarp) {
+      // ================= MMA issue: a warp per block, an elected lane issues, the blocks take turns =================
+      // A thread's MMAs are held up at the tensor pipe (its queue is short), and every wait for a barrier costs a hundred
+      // cycles or more even when it is over: while one warp's MMAs run the other does its waiting.  Turns, because with
+      // free access the two blocks' MMAs interleave, both get their scores at the same time, and then both sit in their
+      // softmax while the tensor cores idle (4660 cycles a tile against 2048 of MMAs).
+      const int blk = warp - kIssuerWarp;
       constexpr uint32_t idesc_s = tc_idesc(kBlockRows, kTileKeys, false, kHalf);
       constexpr uint32_t idesc_o = tc_idesc(kBlockRows, kDim, true, kHalf);
-      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-      const uint32_t q_u32 = smem_u32(qtiles), ring_u32 = smem_u32(ring);
-      auto issue_s = [&](int blk, uint32_t tile) {
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + (uint32_t)blk * kBlockCols;
+      // descriptors: only the address field, the lowest, changes
+      const uint64_t q_desc = tc_desc(smem_u32(qtiles) + (uint32_t)(blk * kQBlockBytes), 16);
+      const uint64_t k_desc = tc_desc(smem_u32(ring), 16, kGroupBytes), v_desc = tc_desc(smem_u32(ring), 1024, kGroupBytes);
+      auto issue_s = [&](int entry) {
+        const uint64_t kd = k_desc + (uint64_t)(uint32_t)(entry * (kTileBytes >> 4));
 #pragma unroll
         for (int ks = 0; ks < kDim / 16; ++ks)
-          tc_mma_f16_ss(tm + (uint32_t)blk * kBlockCols,
-                        tc_desc(q_u32 + (uint32_t)(blk * kQBlockBytes + (ks >> 2) * kQHalfBytes + (ks & 3) * 32), 16),
-                        tc_desc(tile + (uint32_t)((ks >> 2) * 1024 + (ks & 3) * 32), 16, kGroupBytes), idesc_s, ks > 0 ? 1u : 0u);
+          tc_mma_f16_ss(tm, q_desc + (uint64_t)(((ks >> 2) * kQHalfBytes + (ks & 3) * 32) >> 4),
+                        kd + (uint64_t)(((ks >> 2) * 1024 + (ks & 3) * 32) >> 4), idesc_s, ks > 0 ? 1u : 0u);
         tc_commit(&s_ready[blk]);
       };
-      auto issue_o = [&](int blk, int half, uint32_t tile, bool accumulate) {
+      auto issue_o = [&](int half, int entry, bool accumulate) {
+        const uint64_t vd = v_desc + (uint64_t)(uint32_t)(entry * (kTileBytes >> 4));
 #pragma unroll
         for (int x = 0; x < kTileKeys / 32; ++x) {
           const int ks = half * (kTileKeys / 32) + x;
-          tc_mma_f16_ta(tm + (uint32_t)blk * kBlockCols + kOCol, tm + (uint32_t)blk * kBlockCols + (uint32_t)(8 * ks),
-                        tc_desc(tile + (uint32_t)(ks * 2 * kGroupBytes), 1024, kGroupBytes), idesc_o, (accumulate || ks > 0) ? 1u : 0u);
+          tc_mma_f16_ta(tm + kOCol, tm + (uint32_t)(8 * ks), vd + (uint64_t)((ks * 2 * kGroupBytes) >> 4), idesc_o,
+                        (accumulate || ks > 0) ? 1u : 0u);
         }
       };
       // (A wait that gave up is noticed at the end of the tile: what is issued until then works on old data in bounds.)
-      bool ok = true, issued = false;
+      bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         ok = tc_wait(bar, parity, abort_flag) && ok;
         __syncwarp();
         tc_fence_after();
+      };
+      uint32_t turn = blk ^ 1;  // parity of the barrier that says it is this block's turn (block 0 begins)
+      auto take_turn = [&]() { wait(&my_turn[blk], turn); };
+      auto pass_turn = [&]() {
+        if (lane == 0) mbar_arrive(&my_turn[blk ^ 1]);
+        turn ^= 1u;
       };
       int e = 0;        // ring entry, in the order they come: K(0), V(0), K(1), ...
       uint32_t ph = 0;  // and its phase
       auto next_entry = [&]() {
         if (++e == kRing) e = 0, ph ^= 1u;
       };
-      uint32_t seen[2] = {0, 0}, piece = 0;
+      uint32_t seen = 0, piece = 0;
+      bool issued = false;
       for (; ok; ++piece) {
         const Piece* now = peek();
         if (!now) break;
         const int n = now->ntiles, i0 = now->i0, s_tiles = now->s_tiles, m0 = now->m0;
-        int bfirst[2], blast[2], last_seen[2] = {-1, -1};
-        bool begun[2] = {false, false};
-        block_pos(*now, 0, bfirst[0], blast[0]);
-        block_pos(*now, 1, bfirst[1], blast[1]);
+        int bfirst, blast, last_seen = -1;
+        block_pos(*now, blk, bfirst, blast);
         pop();
-        auto sees = [&](int blk, int i) { return block_sees(bfirst[blk], blast[blk], list_row(s_tiles, m0, i0 + i)); };
-#pragma unroll
-        for (int blk = 0; blk < 2; ++blk)
-          for (int i = n - 1; i >= 0 && last_seen[blk] < 0; --i)
-            if (sees(blk, i)) last_seen[blk] = i;
+        auto sees = [&](int i) { return block_sees(bfirst, blast, list_row(s_tiles, m0, i0 + i)); };
+        for (int i = n - 1; i >= 0 && last_seen < 0; --i)
+          if (sees(i)) last_seen = i;
+        bool begun = false, sees_now = sees(0);
         wait(&q_ready, piece & 1u);
         wait(&full[e], ph);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+        take_turn();
         if (elect_one()) {
-#pragma unroll
-          for (int blk = 0; blk < 2; ++blk)
-            if (sees(blk, 0)) issue_s(blk, ring_u32 + (uint32_t)(e * kTileBytes));
+          if (sees_now) issue_s(e);
           tc_commit(&empty[e]);
         }
         __syncwarp();
+        pass_turn();
         issued = true;
         next_entry();
         for (int i = 0; i < n && ok; ++i) {
@@ -650,62 +648,44 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           wait(&full[ve], ph);
           next_entry();
           const int ke = e;
-          const bool more = i + 1 < n;
-          const uint32_t v_tile = ring_u32 + (uint32_t)(ve * kTileBytes), k_tile = ring_u32 + (uint32_t)(ke * kTileBytes);
-#pragma unroll
-          for (int blk = 0; blk < 2; ++blk) {
-            if (sees(blk, i)) {
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                wait(&p_ready[blk][half], seen[blk] & 1u);
-                if (elect_one()) {
-                  issue_o(blk, half, v_tile, begun[blk]);
-                  if (half == 0) tc_commit(&h_done[blk]);
-                  if (half == 1 && i == last_seen[blk]) tc_commit(&o_done[blk]);
-                }
-                __syncwarp();
-              }
-              ++seen[blk];
-              begun[blk] = true;
+          const bool more = i + 1 < n, sees_next = more && sees(i + 1);
+          if (sees_now) wait(&p_ready[blk][0], seen & 1u);
+          take_turn();
+          if (sees_now) {
+            if (elect_one()) {
+              issue_o(0, ve, begun);
+              tc_commit(&h_done[blk]);
             }
-            if (blk == 0 && more) wait(&full[ke], ph);
-            if (more && sees(blk, i + 1)) {  // over the P just consumed: the MMAs of a thread run in order
-              if (elect_one()) issue_s(blk, k_tile);
-              __syncwarp();
+            __syncwarp();
+            wait(&p_ready[blk][1], seen & 1u);
+            if (elect_one()) {
+              issue_o(1, ve, begun);
+              if (i == last_seen) tc_commit(&o_done[blk]);
             }
+            __syncwarp();
+            ++seen;
+            begun = true;
           }
+          if (more) wait(&full[ke], ph);
           if (elect_one()) {
             tc_commit(&empty[ve]);
-            if (more) tc_commit(&empty[ke]);
+            if (sees_next) issue_s(ke);  // over the P just consumed: the MMAs of a thread run in order
           }
           __syncwarp();
-          if (more) next_entry();
+          pass_turn();
+          if (more) {
+            if (elect_one()) tc_commit(&empty[ke]);
+            __syncwarp();
+            next_entry();
+          }
+          sees_now = sees_next;
           ok = __all_sync(0xffffffffu, ok);
         }
       }
       if (!ok && issued) {  // gave up: let the MMAs in flight finish before tensor memory is freed
-        if (elect_one()) tc_commit(&drained);
+        if (elect_one()) tc_commit(&drained[blk]);
         __syncwarp();
-        mbar_wait_bounded(&drained, 0);
-      }
-    } else if (warp == kPieceWarp) {
-      // ================= the pieces of the run =================
-      Pieces pc(s_place[0], s_place[1]);
-      uint32_t ph = 1;  // the first round finds the slots empty
-      bool first = true, any = true;
-      for (int slot = 0; any; first = false) {
-        any = pc.next(ka);
-        if (!tc_wait(&pc_empty[slot], ph, abort_flag)) break;
-        if (lane == 0) {
-          s_piece[slot] = pc.piece(any);
-          mbar_arrive(&pc_full[slot]);
-          // what the join needs: the run's first row tile, whether it began in an earlier run, whether it ends in this one
-          if (first)
-            *record = make_int4(pc.at.b, pc.at.h, pc.at.qt,
-                                any ? (pc.i0 > 0 ? 1 : 0) | (pc.i0 + pc.ntiles == pc.tile.n ? 2 : 0) : 0);
-        }
-        __syncwarp();
-        if (++slot == kPieces) slot = 0, ph ^= 1u;
+        mbar_wait_bounded(&drained[blk], 0);
       }
     } else {
       // ================= K (warp 10) and V (warp 11) tiles =================
@@ -717,14 +697,35 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       int e = is_v;
       uint32_t ph = 1, fixes = 0;  // the first round finds the entries empty
       bool live = true;
+      Pieces walk(s_place[0], s_place[1]);
+      uint32_t slot_ph = 1;  // the first round finds the pieces' slots empty, too
+      bool first = true;
       while (live) {
-        const Piece* now = peek();
-        if (!now) break;
-        const int ntiles = now->ntiles, i0 = now->i0, kv_len = now->kv_len, head = now->h;
-        const int s_tiles = now->s_tiles, m0 = now->m0, rows_hi = now->hi, rows_lo = now->lo, rows_snk = now->snk;
+        Piece now;
+        if (is_v) {
+          const Piece* p = peek();
+          if (!p) break;
+          now = *p;
+          pop();
+        } else {  // warp 10 walks the run and hands out its pieces
+          const bool any = walk.next(ka);
+          now = walk.piece(any);
+          if (!(live = tc_wait(&pc_empty[pc_slot], slot_ph, abort_flag))) break;
+          if (lane == 0) {
+            s_piece[pc_slot] = now;
+            mbar_arrive(&pc_full[pc_slot]);
+            // what the join needs: the run's first row tile, whether it began in an earlier run, whether it ends in this
+            if (first) *record = make_int4(now.b, now.h, walk.at.qt, any ? (now.i0 > 0 ? 1 : 0) | (now.i0 + now.ntiles == walk.tile.n ? 2 : 0) : 0);
+          }
+          __syncwarp();
+          first = false;
+          if (++pc_slot == kPieces) pc_slot = 0, slot_ph ^= 1u;
+          if (!any) break;
+        }
+        const int ntiles = now.ntiles, i0 = now.i0, kv_len = now.kv_len, head = now.h;
+        const int s_tiles = now.s_tiles, m0 = now.m0, rows_hi = now.hi, rows_lo = now.lo, rows_snk = now.snk;
         const unsigned char* base = (is_v ? ka.v_base : ka.k_base) + (size_t)head * kDim * 2;
-        const int* table = a.page_table + (size_t)now->b * a.pages_per_seq;
-        pop();
+        const int* table = a.page_table + (size_t)now.b * a.pages_per_seq;
         // rows some token of the row tile sees
         auto wanted = [&](int lo, int hi) { return lo < rows_hi && (hi > rows_lo || lo < rows_snk); };
         auto page_of = [&](int i) -> int {  // what this lane's copy of tile i reads; -2: nothing (zeros)
