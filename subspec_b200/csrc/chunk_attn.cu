@@ -48,12 +48,13 @@ namespace {
 // multiple of 8), instead of one copy per half.
 //
 // Tensor memory: per block 256 columns, S | O, 128 each (O: head_dim).
-constexpr int kTileKeys = 128;
+constexpr int kTileKeys = 128, kHalfKeys = kTileKeys / 2;
 constexpr int kBlockRows = 128;
 constexpr int kCtaRows = 2 * kBlockRows;
 constexpr int kRing = 5;
-constexpr int kChunkThreads = 384;
-constexpr int kIssuerWarp = 8, kLoadWarp = 10;
+constexpr int kSoftmaxWarps = 16;
+constexpr int kChunkThreads = 32 * (kSoftmaxWarps + 4);
+constexpr int kIssuerWarp = kSoftmaxWarps, kLoadWarp = kIssuerWarp + 2;
 constexpr uint32_t kBlockCols = 256, kOCol = 128;
 #ifndef KFMA
 #define KFMA 8
@@ -66,6 +67,21 @@ constexpr int kGroups = 36;    // groups of requests whose costs are summed up s
 template <int kDim>
 constexpr size_t tc_smem() {
   return (size_t)kCtaRows * kDim * 2 + (size_t)kRing * kTileKeys * kDim * 2 + 1024;
+}
+
+// The two warps of a row: a barrier, and one that tells both whether either has a thread with `x`.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool pair_or(int id, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, %2, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)x), "r"(id)
+      : "memory");
+  return r != 0;
 }
 
 // First cache row of entry i of a tile list.
@@ -200,7 +216,7 @@ struct Piece {
   int s_tiles, m0, hi, lo, snk;  // the list (TileList)
 };
 constexpr int kPieces = 4;  // in flight
-constexpr int kPieceReaders = 11;
+constexpr int kPieceReaders = kSoftmaxWarps + 3;
 
 struct Pieces {
   Place at, end;  // the run ends in front of `end`
@@ -250,8 +266,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     chunk_attn_tc_kernel(const ChunkArgs ka, const __grid_constant__ CUtensorMap tmap_k,
                          const __grid_constant__ CUtensorMap tmap_v) {
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t full[kRing], empty[kRing], s_ready[2], p_ready[2][2], h_done[2], o_done[2], my_turn[2], q_ready, fix, drained[2], pc_full[kPieces], pc_empty[kPieces];
-  __shared__ long long s_cost[kGroups];
+  __shared__ __align__(8) uint64_t full[kRing], empty[kRing], s_ready[2], p_ready[2], o_done[2], my_turn[2], q_ready, fix, drained[2], pc_full[kPieces], pc_empty[kPieces];
+  __shared__ union {
+    long long cost[kGroups];  // of the groups of requests; then
+    float row[kCtaRows];      // what the two warps of a row tell each other
+  } s_words;
+  __shared__ uint32_t s_move[8];  // per pair of warps: the tile in front of which the reference points are to move
   __shared__ Place s_place[2];
   __shared__ Piece s_piece[kPieces];
   __shared__ uint32_t s_tmem;
@@ -274,7 +294,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const int group_size = (a.batch + kGroups - 1) / kGroups;
   for (int g = warp; g < kGroups; g += kChunkThreads / 32) {
     const long long c = requests_cost(ka, min(g * group_size, a.batch), min((g + 1) * group_size, a.batch));
-    if (lane == 0) s_cost[g] = c;
+    if (lane == 0) s_words.cost[g] = c;
   }
   unsigned char* qtiles = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   unsigned char* ring = qtiles + 2 * kQBlockBytes;
@@ -285,14 +305,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
     for (int k = 0; k < 2; ++k) {
       mbar_init(&s_ready[k], 1);
-      mbar_init(&p_ready[k][0], 4);
-      mbar_init(&p_ready[k][1], 4);
-      mbar_init(&h_done[k], 1);
+      mbar_init(&p_ready[k], kSoftmaxWarps / 2);
       mbar_init(&o_done[k], 1);
       mbar_init(&my_turn[k], 1);
       mbar_init(&drained[k], 1);
     }
-    mbar_init(&q_ready, 8);
+    mbar_init(&q_ready, kSoftmaxWarps);
     for (int k = 0; k < kPieces; ++k) {
       mbar_init(&pc_full[k], 1);
       mbar_init(&pc_empty[k], kPieceReaders);
@@ -300,10 +318,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     mbar_init(&fix, 1);
     mbar_init_fence();
     s_abort = 0;
+    for (int k = 0; k < 8; ++k) s_move[k] = 0xffffffffu;
   }
   __syncthreads();
   long long total = 0;
-  for (int g = 0; g < kGroups; ++g) total += s_cost[g];
+  for (int g = 0; g < kGroups; ++g) total += s_words.cost[g];
   total *= a.num_kv_heads;
   const int runs = (int)max(1LL, min((long long)gridDim.x, total / kMinRun));
   int4* record = ka.runs + run;
@@ -314,7 +333,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   }
   if (warp < 2) {
     const int c = run + warp;
-    const Place p = c < runs ? locate(ka, c * total / runs, s_cost, group_size) : Place{a.batch, 0, 0, 0};
+    const Place p = c < runs ? locate(ka, c * total / runs, s_words.cost, group_size) : Place{a.batch, 0, 0, 0};
     if (lane == 0) s_place[warp] = p;
   }
   if (warp == kIssuerWarp) {
@@ -353,30 +372,50 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     return t0 + kTileKeys - 1 <= first && (a.window == 0 || t0 > last - a.window || t0 + kTileKeys <= a.sinks);
   };
 
-  if (warp < 8) {
+  if (warp < kSoftmaxWarps) {
     // ================= softmax =================
-    const int blk = warp >> 2, rr = (int)threadIdx.x & 127;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int blk = warp >> 3, half = (warp >> 2) & 1, rr = (warp & 3) * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)blk * kBlockCols;
-    const uint32_t o_addr = lane_base + kOCol;
+    const uint32_t s_addr = lane_base + (uint32_t)(half * kHalfKeys);
+    const uint32_t o_addr = lane_base + kOCol + (uint32_t)(half * (kDim / 2));  // its half of the dims, too
     const float c2 = ka.scale_log2;
     const uint64_t c2p = f2_pack(c2, c2);
     // fp16 weights sit 2^7 higher, out of the subnormals
     constexpr float kOffset = kHalf ? 7.f : 0.f;
-    constexpr float kSumLimit = kHalf ? 32768.f : 1.0995116e12f;
+    // Weights need a reference point near the row's maximum, not the maximum itself, and every weight is positive, so that
+    // the sum of a tile's tells whether any is too large: no tile but a row's first is searched for its maximum.
+    // bf16 (and the fp32 sums) hold weights of up to 2^100 as well as 1.  A tile that passes 2^40 makes the reference point
+    // move in front of the next tile; one that passes 2^100 (scores that rise by 69 beyond a row's reference within one
+    // tile) spoils the row, which is done over at the end.
+    // fp16 holds 2^15: there a tile that does not fit is done again at once, against its own maximum.
+    constexpr float kSumLimit = kHalf ? 32768.f : 1.0995116e12f, kSpoilt = 1.2676506e30f;
+    const int pair = 1 + blk * 4 + (warp & 3);  // the named barrier of the two warps with these rows
+    float& word = s_words.row[blk * kBlockRows + rr];
+    // x of the one and of the other, put together by the second
+    auto exchange = [&](float x, auto&& join) {
+      if (half == 0) word = x;
+      pair_sync(pair);
+      if (half == 1) word = x = join(x, word);
+      pair_sync(pair);
+      return half == 0 ? word : x;
+    };
     uint32_t seen = 0, finished = 0;  // tiles, and pieces with any, that this block has worked on
-    // Every thread brings its own row of Q of a piece (a row that does not exist: zeros) ...
+    // Every thread brings half of its row of Q of a piece (a row that does not exist: zeros) ...
     auto load_q = [&](const Piece& pc) {
-      const int row = pc.row0 + (int)threadIdx.x, tok = row / G;
+      const int row = pc.row0 + blk * kBlockRows + rr, tok = row / G;
       const bool ok = row < pc.rows;
       const unsigned char* src = reinterpret_cast<const unsigned char*>(a.q);
       if (ok) src += 2 * ((size_t)(pc.q0 + tok) * a.q_token_stride + (size_t)(pc.h * G + row - tok * G) * a.q_head_stride);
       unsigned char* d = qtiles + blk * kQBlockBytes + rr * 128;
 #pragma unroll
-      for (int c = 0; c < kDim / 8; ++c)
-        cp_async16(d + (c >> 3) * kQHalfBytes + (((c & 7) ^ (rr & 7)) << 4), src + c * 16, ok ? 16 : 0);
+      for (int x = 0; x < kDim / 16; ++x) {
+        const int c = half * (kDim / 16) + x;
+        cp_async16(d + (c >> 3) * kQHalfBytes + (((c & 7) ^ (rr & 7)) << 4), src + (ok ? c * 16 : 0), ok ? 16 : 0);
+      }
       cp_async_commit();
     };
-    auto hand_q = [&]() {  // ... and the issuer may read it
+    auto hand_q = [&]() {  // ... and the issuers may read it
       cp_async_wait<0>();
       fence_async_smem();
       __syncwarp();
@@ -389,8 +428,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
     while (live) {
       const Piece* now = peek();
-      if (!now) break;
-      const int row = now->row0 + (int)threadIdx.x;
+      if (pair_or(pair, now == nullptr)) break;  // (both or neither: they meet at barriers)
+      const int row = now->row0 + blk * kBlockRows + rr;
       const bool row_ok = row < now->rows, block_ok = now->row0 + blk * kBlockRows < now->rows, whole = now->whole;
       const int tok = row / G, head = now->h * G + row - tok * G, t = now->q0 + tok, b = now->b;
       int bfirst, blast;
@@ -399,131 +438,154 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const int ntiles = now->ntiles, i0 = now->i0, s_tiles = now->s_tiles, m0 = now->m0;
       pop();
       float m = -INFINITY, l = 0.f;
-      uint32_t done = 0;  // tiles of this piece
+      uint32_t done = 0;       // tiles of this piece
+      bool all_begun = false;  // no row of the warp without a reference point
       for (int i = 0; i < ntiles; ++i) {
         const int t0 = list_row(s_tiles, m0, i0 + i);
         if (!block_sees(bfirst, blast, t0)) continue;
-        live = __all_sync(0xffffffffu, tc_wait(&s_ready[blk], seen & 1u, abort_flag));
-        if (!live) break;
+        live = tc_wait(&s_ready[blk], seen & 1u, abort_flag);
+        __syncwarp();
         tc_fence_after();
-        // Half a tile (64 scores) at a time in registers: all 128 would fill them and leave the compiler nothing to
-        // reorder with.  The second half's scores stay in tensor memory until the first half's P is done.
-        uint32_t r[2][32];
-        tmem_ld32_async(lane_base, r[0]);
-        tmem_ld32_async(lane_base + 32, r[1]);
         const bool masked = !block_sees_all(bfirst, blast, t0);
-        auto hide = [&](uint32_t (&x)[32], int c) {
-          const int p0 = t0 + 32 * c;
+        auto hide = [&](int c, uint32_t (&r)[32]) {
+          const int p0 = t0 + half * kHalfKeys + 32 * c;
           uint32_t bits = bits_below(pos + 1 - p0);
           if (a.window > 0) bits &= ~bits_below(pos - a.window + 1 - p0) | bits_below(a.sinks - p0);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] = (bits >> j) & 1u ? x[j] : 0xff800000u;
+          for (int j = 0; j < 32; ++j) r[j] = (bits >> j) & 1u ? r[j] : 0xff800000u;
         };
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          tmem_wait_ld_dep(r[0]);
-          tmem_wait_ld_dep(r[1]);
-          if (masked) hide(r[0], 2 * half), hide(r[1], 2 * half + 1);
-          // Weights need a reference point near the row's maximum, not the maximum itself: a tile is first tried against
-          // the old one, without looking for its maximum.  Every weight is positive, so a sum within kSumLimit proves that
-          // none is too large (for the 16-bit type and the fp32 sums); anything else (a larger sum, an overflow, NaN, a row
-          // that has seen nothing yet) moves the reference point to the maximum of the scores not yet handed over, rescales
-          // O and does the half tile again.
-          bool move = half == 0 && m == -INFINITY, moved = false;
-          uint32_t pk[2][16];
-          float sum;
-          for (;;) {
-            if (__any_sync(0xffffffffu, move)) {
-              moved = true;
-              float top = m, alpha = 1.f;
-              for (int c = 2 * half; c < 4; ++c) {  // NaN stays NaN: a NaN score makes the row NaN
-                uint32_t x[32];
-                tmem_ld32_async(lane_base + 32 * c, x);
-                tmem_wait_ld_dep(x);
-                if (masked) hide(x, c);
-                float mx = __uint_as_float(x[0]);
-#pragma unroll
-                for (int j = 1; j < 31; j += 2) mx = max3_nan(mx, __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
-                top = max3_nan(top, max3_nan(mx, __uint_as_float(x[31]), mx) * c2, top);  // c2 > 0
-              }
-              if (move) {
-                alpha = m == -INFINITY ? 0.f : ex2f(m - top);
-                m = top;
-              }
-              if (half == 1) {  // O is at rest only when the first half's MMAs have landed
-                live = __all_sync(0xffffffffu, tc_wait(&h_done[blk], seen & 1u, abort_flag));
-                tc_fence_after();
-              }
-              if ((done > 0 || half == 1) && __any_sync(0xffffffffu, alpha != 1.f)) {
+        auto rescale_o = [&](float alpha) {  // this warp's half of the dims
+          // (O is complete up to the tile before: its MMAs were committed together with this tile's scores)
+          if (done == 0 || !__any_sync(0xffffffffu, alpha != 1.f)) return;
 #pragma unroll 1
-                for (int c = 0; c < kDim / 32; ++c) {
-                  uint32_t rc[32];
-                  tmem_ld32_async(o_addr + 32 * c, rc);
-                  tmem_wait_ld_dep(rc);
+          for (int c = 0; c < kDim / 64; ++c) {
+            uint32_t rc[32];
+            tmem_ld32_async(o_addr + 32 * c, rc);
+            tmem_wait_ld_dep(rc);
 #pragma unroll
-                  for (int j = 0; j < 32; ++j) rc[j] = __float_as_uint(__uint_as_float(rc[j]) * alpha);
-                  tmem_st32(o_addr + 32 * c, rc);
-                }
-              }
-              l *= alpha;
-            }
-            const float u = m == -INFINITY ? 0.f : m - kOffset;  // (-inf: every score is -inf, every weight 0)
-            const uint64_t nup = f2_pack(-u, -u);
-            uint64_t sm2[4] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f), f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                float x0, x1, p0, p1;
-                f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c][2 * j]), __uint_as_float(r[c][2 * j + 1])), c2p, nup), x0, x1);
-                if (j % kFmaEvery == kFmaEvery - 1) {
-                  exp2_pair(x0, x1, p0, p1);  // some pairs on the FMA pipe
-                } else {
-                  p0 = ex2f(x0);
-                  p1 = ex2f(x1);
-                }
-                sm2[j & 3] = f2_add(sm2[j & 3], f2_pack(p0, p1));
-                pk[c][j] = pack16<kHalf>(p0, p1);
-              }
-            }
-            float e0, e1;
-            f2_unpack(f2_add(f2_add(sm2[0], sm2[1]), f2_add(sm2[2], sm2[3])), e0, e1);
-            sum = e0 + e1;
-            move = !(sum <= kSumLimit);
-            if (moved || !__any_sync(0xffffffffu, move)) break;
+            for (int j = 0; j < 32; ++j) rc[j] = __float_as_uint(__uint_as_float(rc[j]) * alpha);
+            tmem_st32(o_addr + 32 * c, rc);
           }
-          if (half == 0) {
-            tmem_ld32_async(lane_base + 64, r[0]);
-            tmem_ld32_async(lane_base + 96, r[1]);
+        };
+        // The reference points of the rows go to the tile's maximum: of those that have none yet, or of all.
+        auto move_to_max = [&](bool all) {
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {  // NaN stays NaN: a NaN score makes the row NaN
+            uint32_t r[32];
+            tmem_ld32_async(s_addr + 32 * c, r);
+            tmem_wait_ld_dep(r);
+            if (masked) hide(c, r);
+            float mx = __uint_as_float(r[0]);
+#pragma unroll
+            for (int j = 1; j < 31; j += 2) mx = max3_nan(mx, __uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+            top = max3_nan(top, mx, __uint_as_float(r[31]));
           }
-          l += sum;
-          tmem_st16(lane_base + 32 * half, pk[0]);
-          tmem_st16(lane_base + 32 * half + 16, pk[1]);
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_ready[blk][half]);  // this half's share of O += P V can begin
+          top = exchange(top * c2, [](float x, float y) { return max3_nan(x, y, y); });  // c2 > 0
+          float alpha = 1.f;
+          if (all || m == -INFINITY) {
+            const float m_new = max3_nan(m, top, top);
+            alpha = m == -INFINITY ? 0.f : ex2f(m - m_new);
+            m = m_new;
+            l *= alpha;
+          }
+          all_begun = __all_sync(0xffffffffu, m != -INFINITY);
+          rescale_o(alpha);
+        };
+        if (!all_begun && __any_sync(0xffffffffu, m == -INFINITY)) move_to_max(false);
+        if (!kHalf && s_move[pair - 1] == seen) {
+          // 2^k past the reference point in sum: it moves up by k
+          const float both = exchange(l, [](float x, float y) { return x + y; });
+          const int k = both > 1.f && both < kSpoilt ? (__float_as_int(both) >> 23) - 127 : 0;
+          const float alpha = __int_as_float((127 - k) << 23);
+          m += (float)k;
+          l *= alpha;
+          rescale_o(alpha);
         }
-        if (!live) break;
+        bool moved = false;
+        float sum;
+        for (;;) {
+          const float u = m == -INFINITY ? 0.f : m - kOffset;  // (-inf: every score is -inf, every weight 0)
+          const uint64_t nup = f2_pack(-u, -u);
+          uint64_t sm2[4] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f), f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+          uint32_t pk[2][16];
+          auto weights = [&](uint32_t (&r)[32], uint32_t (&pk)[16]) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              float x0, x1, p0, p1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), c2p, nup), x0, x1);
+              if (j % kFmaEvery == kFmaEvery - 1) {
+                exp2_pair(x0, x1, p0, p1);  // some pairs on the FMA pipe
+              } else {
+                p0 = ex2f(x0);
+                p1 = ex2f(x1);
+              }
+              sm2[j & 3] = f2_add(sm2[j & 3], f2_pack(p0, p1));
+              pk[j] = pack16<kHalf>(p0, p1);
+            }
+          };
+          uint32_t ra[32], rb[32];
+          tmem_ld32_async(s_addr, ra);
+          tmem_wait_ld_dep(ra);
+          tmem_ld32_async(s_addr + 32, rb);  // (a load takes 100 to 300 cycles beside the MMAs: under the first's arithmetic)
+          if (masked) hide(0, ra);
+          weights(ra, pk[0]);
+          tmem_wait_ld_dep(rb);
+          if (!kHalf) tmem_st16(s_addr, pk[0]);  // over this warp's own scores, which are all in registers
+          if (masked) hide(1, rb);
+          weights(rb, pk[1]);
+          if (!kHalf) tmem_st16(s_addr + 16, pk[1]);
+          float e0, e1;
+          f2_unpack(f2_add(f2_add(sm2[0], sm2[1]), f2_add(sm2[2], sm2[3])), e0, e1);
+          sum = e0 + e1;
+          if (kHalf) {  // both warps of a row together: what one finds the other hears
+            if (pair_or(pair, !(sum <= kSumLimit) || !live)) {
+              live = !pair_or(pair, !live);
+              if (!moved && live) {
+                moved = true;
+                move_to_max(true);
+                continue;
+              }
+            }
+            tmem_st16(s_addr, pk[0]);
+            tmem_st16(s_addr + 16, pk[1]);
+          }
+          break;
+        }
+        if (!kHalf) {
+          if (__any_sync(0xffffffffu, !(sum <= kSumLimit)) && lane == 0) s_move[pair - 1] = seen + 1;
+          if (sum > kSpoilt) sum = INFINITY;
+        }
+        l += sum;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[blk]);
         ++done;
         ++seen;
+        if (!live) break;
       }
+      live = !pair_or(pair, !live);
+      l = exchange(l, [](float x, float y) { return x + y; });
       // The block's Q has served its last scores: the next piece's comes while the last MMAs run.
       const Piece* following = live ? peek() : nullptr;
       if (following) load_q(*following);
       // ---- the result: O / l, or the part as it is ----
       if (live && done > 0) live = __all_sync(0xffffffffu, tc_wait(&o_done[blk], finished++ & 1u, abort_flag));
       if (following) hand_q();
+      live = !pair_or(pair, !live);
       if (!live) break;
       if (!block_ok) continue;
       tc_fence_after();
       const float inv = l != 0.f ? 1.f / l : 0.f;
       bool odd = false;  // a value that is not finite although the sum of the weights is
-      const size_t prow = ((size_t)2 * run + (i0 == 0 ? 1 : 0)) * kCtaRows + threadIdx.x;
-      uint16_t* out_row = reinterpret_cast<uint16_t*>(a.out) + (size_t)t * a.o_token_stride + (size_t)head * a.o_head_stride;
-      if (!whole && row_ok) reinterpret_cast<float2*>(ka.part_ml)[prow] = make_float2(m, l);
+      const size_t prow = ((size_t)2 * run + (i0 == 0 ? 1 : 0)) * kCtaRows + blk * kBlockRows + rr;
+      uint16_t* out_row = reinterpret_cast<uint16_t*>(a.out) + (size_t)t * a.o_token_stride + (size_t)head * a.o_head_stride +
+                          half * (kDim / 2);
+      float* part_row = ka.part_o + prow * kDim + half * (kDim / 2);
+      if (!whole && row_ok && half == 0) reinterpret_cast<float2*>(ka.part_ml)[prow] = make_float2(m, l);
 #pragma unroll
-      for (int c = 0; c < kDim / 32; ++c) {
+      for (int c = 0; c < kDim / 64; ++c) {
         uint32_t rc[32];
         if (done > 0) {
           tmem_ld32_async(o_addr + 32 * c, rc);
@@ -536,8 +598,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (row_ok) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              reinterpret_cast<uint4*>(ka.part_o + prow * kDim)[8 * c + j] =
-                  make_uint4(rc[4 * j], rc[4 * j + 1], rc[4 * j + 2], rc[4 * j + 3]);
+              reinterpret_cast<uint4*>(part_row)[8 * c + j] = make_uint4(rc[4 * j], rc[4 * j + 1], rc[4 * j + 2], rc[4 * j + 3]);
           }
         } else {
 #pragma unroll
@@ -560,17 +621,23 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
       }
       tc_fence_before();
-      // 0 * inf from a V row that this row does not see but others of the tile do, or scores of -inf alone: such rows
-      // are done over key by key.  (A NaN sum comes from scores the row sees: NaN is the result.)
-      uint32_t again = __ballot_sync(0xffffffffu, whole && row_ok && l == l && (odd || (l == 0.f && pos >= 0)));
-      while (again) {
-        const int src = __ffs(again) - 1;
-        again &= again - 1;
-        attn_row<kHalf, kDim>(ka, b, __shfl_sync(0xffffffffu, pos, src), __shfl_sync(0xffffffffu, t, src),
-                              __shfl_sync(0xffffffffu, head, src));
+      // 0 * inf from a V row that this row does not see but others of the tile do, or scores of -inf alone: such rows are
+      // done over key by key, whole, after the other half of the dims has been written.  (A NaN sum comes from scores the
+      // row sees: NaN is the result; an infinite one says that the row is spoilt.)
+      const bool bad = whole && row_ok && l == l && (odd || l == INFINITY || (l == 0.f && pos >= 0));
+      if (pair_or(pair, bad)) {
+        uint32_t again = __ballot_sync(0xffffffffu, exchange(bad ? 1.f : 0.f, [](float x, float y) { return x + y; }) > 0.f);
+        again &= half ? 0xffff0000u : 0xffffu;  // the two warps share them out
+        while (again) {
+          const int src = __ffs(again) - 1;
+          again &= again - 1;
+          attn_row<kHalf, kDim>(ka, b, __shfl_sync(0xffffffffu, pos, src), __shfl_sync(0xffffffffu, t, src),
+                                __shfl_sync(0xffffffffu, head, src));
+        }
       }
     }
   } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp < kLoadWarp) {
       // ================= MMA issue: a warp per block, an elected lane issues, the blocks take turns =================
       // A thread's MMAs are held up at the tensor pipe (its queue is short), and every wait for a barrier costs a hundred
@@ -592,14 +659,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                         kd + (uint64_t)(((ks >> 2) * 1024 + (ks & 3) * 32) >> 4), idesc_s, ks > 0 ? 1u : 0u);
         tc_commit(&s_ready[blk]);
       };
-      auto issue_o = [&](int half, int entry, bool accumulate) {
+      auto issue_o = [&](int entry, bool accumulate) {
         const uint64_t vd = v_desc + (uint64_t)(uint32_t)(entry * (kTileBytes >> 4));
 #pragma unroll
-        for (int x = 0; x < kTileKeys / 32; ++x) {
-          const int ks = half * (kTileKeys / 32) + x;
-          tc_mma_f16_ta(tm + kOCol, tm + (uint32_t)(8 * ks), vd + (uint64_t)((ks * 2 * kGroupBytes) >> 4), idesc_o,
-                        (accumulate || ks > 0) ? 1u : 0u);
-        }
+        for (int ks = 0; ks < kTileKeys / 16; ++ks)  // 16 cache rows = 8 columns of P; a half's P begins where its scores did
+          tc_mma_f16_ta(tm + kOCol, tm + (uint32_t)((ks >> 2) * kHalfKeys + 8 * (ks & 3)), vd + (uint64_t)((ks * 2 * kGroupBytes) >> 4),
+                        idesc_o, (accumulate || ks > 0) ? 1u : 0u);
       };
       // (A wait that gave up is noticed at the end of the tile: what is issued until then works on old data in bounds.)
       bool ok = true;
@@ -645,29 +710,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         next_entry();
         for (int i = 0; i < n && ok; ++i) {
           const int ve = e;
-          wait(&full[ve], ph);
+          const uint32_t vph = ph;
           next_entry();
           const int ke = e;
-          const bool more = i + 1 < n, sees_next = more && sees(i + 1);
-          if (sees_now) wait(&p_ready[blk][0], seen & 1u);
-          take_turn();
-          if (sees_now) {
-            if (elect_one()) {
-              issue_o(0, ve, begun);
-              tc_commit(&h_done[blk]);
-            }
-            __syncwarp();
-            wait(&p_ready[blk][1], seen & 1u);
-            if (elect_one()) {
-              issue_o(1, ve, begun);
+          const bool more = i + 1 < n;
+          // (Asking a barrier takes 160 cycles even when the answer is yes: these three answers come together.)
+          const bool v_there = mbar_test_wait(&full[ve], vph), k_there = !more || mbar_test_wait(&full[ke], ph);
+          const bool p_there = !sees_now || mbar_test_wait(&p_ready[blk], seen & 1u);
+          const bool sees_next = more && sees(i + 1);
+          if (!v_there) ok = tc_wait(&full[ve], vph, abort_flag) && ok;
+          if (!k_there) ok = tc_wait(&full[ke], ph, abort_flag) && ok;
+          take_turn();  // (comes while P is still being made)
+          if (!p_there) ok = tc_wait(&p_ready[blk], seen & 1u, abort_flag) && ok;
+          __syncwarp();
+          tc_fence_after();
+          if (elect_one()) {
+            if (sees_now) {
+              issue_o(ve, begun);
               if (i == last_seen) tc_commit(&o_done[blk]);
             }
-            __syncwarp();
-            ++seen;
-            begun = true;
-          }
-          if (more) wait(&full[ke], ph);
-          if (elect_one()) {
             tc_commit(&empty[ve]);
             if (sees_next) issue_s(ke);  // over the P just consumed: the MMAs of a thread run in order
           }
@@ -678,6 +739,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             __syncwarp();
             next_entry();
           }
+          seen += sees_now;
+          begun = begun || sees_now;
           sees_now = sees_next;
           ok = __all_sync(0xffffffffu, ok);
         }
@@ -845,6 +908,7 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkArgs ka) {
       mstar = max3_nan(mstar, y, y);
     }
     float acc[kPer] = {}, lsum = 0.f;
+    bool odd = false;
 #pragma unroll 4
     for (int c = c0; c <= c1; ++c) {
       const float2 ml = reinterpret_cast<const float2*>(ka.part_ml)[part(c)];
@@ -852,13 +916,17 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkArgs ka) {
 #pragma unroll
       for (int x = 0; x < kPer; ++x) o[x] = ka.part_o[part(c) * kDim + lane * kPer + x];
       if (ml.y == 0.f) continue;  // nothing seen in this part
+      if (ml.y == INFINITY) {  // spoilt
+        odd = true;
+        continue;
+      }
       const float w = ex2f(ml.x - mstar);
 #pragma unroll
       for (int x = 0; x < kPer; ++x) acc[x] += w * o[x];
       lsum += w * ml.y;
     }
     const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
-    bool odd = lsum == 0.f;
+    odd = odd || lsum == 0.f;
 #pragma unroll
     for (int c = 0; c < kPer; ++c) {
       acc[c] *= inv;
