@@ -69,6 +69,13 @@ constexpr size_t tc_smem() {
   return (size_t)kCtaRows * kDim * 2 + (size_t)kRing * kTileKeys * kDim * 2 + 1024;
 }
 
+// A sector: 32 bytes to an address that is a multiple of 32.
+__device__ __forceinline__ void store32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // The two warps of a row: a barrier, and one that tells both whether either has a thread with `x`.
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ bool pair_or(int id, bool x) {
@@ -266,7 +273,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     chunk_attn_tc_kernel(const ChunkArgs ka, const __grid_constant__ CUtensorMap tmap_k,
                          const __grid_constant__ CUtensorMap tmap_v) {
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t full[kRing], empty[kRing], s_ready[2], p_ready[2], o_done[2], my_turn[2], q_ready, fix, drained[2], pc_full[kPieces], pc_empty[kPieces];
+  __shared__ __align__(8) uint64_t full[kRing], empty[kRing], s_ready[2], p_ready[2], o_done[2], my_turn[2], q_ready[2], fix, drained[2], pc_full[kPieces], pc_empty[kPieces];
   __shared__ union {
     long long cost[kGroups];  // of the groups of requests; then
     float row[kCtaRows];      // what the two warps of a row tell each other
@@ -307,10 +314,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       mbar_init(&s_ready[k], 1);
       mbar_init(&p_ready[k], kSoftmaxWarps / 2);
       mbar_init(&o_done[k], 1);
+      mbar_init(&q_ready[k], kSoftmaxWarps / 2);
       mbar_init(&my_turn[k], 1);
       mbar_init(&drained[k], 1);
     }
-    mbar_init(&q_ready, kSoftmaxWarps);
     for (int k = 0; k < kPieces; ++k) {
       mbar_init(&pc_full[k], 1);
       mbar_init(&pc_empty[k], kPieceReaders);
@@ -401,26 +408,34 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       return half == 0 ? word : x;
     };
     uint32_t seen = 0, finished = 0;  // tiles, and pieces with any, that this block has worked on
-    // Every thread brings half of its row of Q of a piece (a row that does not exist: zeros) ...
+    // The warps of a block bring its rows of Q of a piece, sixteen each (rows that do not exist: zeros): neighbouring lanes
+    // bring neighbouring chunks.  (A row per thread makes 32 scattered accesses of every instruction: 3500 cycles.)
     auto load_q = [&](const Piece& pc) {
-      const int row = pc.row0 + blk * kBlockRows + rr, tok = row / G;
-      const bool ok = row < pc.rows;
-      const unsigned char* src = reinterpret_cast<const unsigned char*>(a.q);
-      if (ok) src += 2 * ((size_t)(pc.q0 + tok) * a.q_token_stride + (size_t)(pc.h * G + row - tok * G) * a.q_head_stride);
-      unsigned char* d = qtiles + blk * kQBlockBytes + rr * 128;
+      constexpr int kChunks = kDim / 8, kPass = 32 / kChunks;  // chunks of a row, rows at once
+      const int c = lane % kChunks, r0 = (warp & 7) * 16 + lane / kChunks;
+      int row = pc.row0 + blk * kBlockRows + r0, tok = row / G, g = row - tok * G;
+      unsigned char* d = qtiles + blk * kQBlockBytes + (c >> 3) * kQHalfBytes;
 #pragma unroll
-      for (int x = 0; x < kDim / 16; ++x) {
-        const int c = half * (kDim / 16) + x;
-        cp_async16(d + (c >> 3) * kQHalfBytes + (((c & 7) ^ (rr & 7)) << 4), src + (ok ? c * 16 : 0), ok ? 16 : 0);
+      for (int x = 0; x < 16; x += kPass) {
+        const int r = r0 + x;
+        const bool ok = row < pc.rows;
+        const unsigned char* src = reinterpret_cast<const unsigned char*>(a.q);
+        if (ok) src += 2 * ((size_t)(pc.q0 + tok) * a.q_token_stride + (size_t)(pc.h * G + g) * a.q_head_stride) + c * 16;
+        cp_async16(d + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, ok ? 16 : 0);
+        row += kPass;
+        g += kPass;
+        while (g >= G) g -= G, ++tok;
       }
       cp_async_commit();
     };
-    auto hand_q = [&]() {  // ... and the issuers may read it
+    auto hand_q = [&]() {  // ... and the block's issuer may read it
       cp_async_wait<0>();
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_ready);
+      if (lane == 0) mbar_arrive(&q_ready[blk]);
     };
+    // whether every row of the output begins on a sector
+    const bool wide_out = !((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(2 * a.o_token_stride) | (uintptr_t)(2 * a.o_head_stride)) & 31u);
     bool live = true;
     if (const Piece* first = peek()) {
       load_q(*first);
@@ -597,8 +612,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (!whole) {
           if (row_ok) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              reinterpret_cast<uint4*>(part_row)[8 * c + j] = make_uint4(rc[4 * j], rc[4 * j + 1], rc[4 * j + 2], rc[4 * j + 3]);
+            for (int j = 0; j < 4; ++j) store32(part_row + 32 * c + 8 * j, &rc[8 * j]);
           }
         } else {
 #pragma unroll
@@ -608,14 +622,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             rc[j] = __float_as_uint(x);
           }
           if (row_ok) {
+            uint32_t v[16];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint4 v;
-              v.x = pack16<kHalf>(__uint_as_float(rc[8 * j]), __uint_as_float(rc[8 * j + 1]));
-              v.y = pack16<kHalf>(__uint_as_float(rc[8 * j + 2]), __uint_as_float(rc[8 * j + 3]));
-              v.z = pack16<kHalf>(__uint_as_float(rc[8 * j + 4]), __uint_as_float(rc[8 * j + 5]));
-              v.w = pack16<kHalf>(__uint_as_float(rc[8 * j + 6]), __uint_as_float(rc[8 * j + 7]));
-              reinterpret_cast<uint4*>(out_row)[4 * c + j] = v;
+            for (int j = 0; j < 16; ++j) v[j] = pack16<kHalf>(__uint_as_float(rc[2 * j]), __uint_as_float(rc[2 * j + 1]));
+            if (wide_out) {
+              store32(out_row + 32 * c, v);
+              store32(out_row + 32 * c + 16, v + 8);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                reinterpret_cast<uint4*>(out_row)[4 * c + j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
             }
           }
         }
@@ -697,7 +713,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         for (int i = n - 1; i >= 0 && last_seen < 0; --i)
           if (sees(i)) last_seen = i;
         bool begun = false, sees_now = sees(0);
-        wait(&q_ready, piece & 1u);
+        wait(&q_ready[blk], piece & 1u);
         wait(&full[e], ph);
         take_turn();
         if (elect_one()) {
@@ -987,8 +1003,9 @@ static void chunk_sizes(ChunkArgs& ka) {
 
 // Scratch: the runs' records (both kernels'), then the parts of the one, then those of the other.
 static size_t part_floats(const ChunkArgs& ka) { return (size_t)2 * ka.ctas * kCtaRows * (ka.a.head_dim + 2); }
+static size_t run_bytes(const ChunkArgs& ka) { return (size_t)ka.ctas * sizeof(int4) + 32; }  // up to a multiple of 32
 static size_t chunk_scratch_bytes(const ChunkArgs& ka) {
-  return (size_t)ka.ctas * sizeof(int4) + part_floats(ka) * sizeof(float) + (ka.few_rows ? chunk_few_scratch_bytes(ka) : 0);
+  return run_bytes(ka) + part_floats(ka) * sizeof(float) + (ka.few_rows ? chunk_few_scratch_bytes(ka) : 0);
 }
 
 extern "C" int subspec_chunk_attention_scratch_bytes(const subspec_chunk_attn_args* args, size_t* bytes) {
@@ -1071,7 +1088,7 @@ extern "C" int subspec_chunk_attention_paged(const subspec_chunk_attn_args* args
   const size_t need = chunk_scratch_bytes(ka);
   if (need && (!a.scratch || (reinterpret_cast<uintptr_t>(a.scratch) & 15u) || a.scratch_bytes < need)) return SUBSPEC_ESCRATCH;
   ka.runs = reinterpret_cast<int4*>(a.scratch);
-  ka.part_o = reinterpret_cast<float*>(ka.runs + ka.ctas);
+  ka.part_o = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(ka.runs + ka.ctas) + 31) & ~(uintptr_t)31);
   ka.part_ml = ka.part_o + (size_t)2 * ka.ctas * kCtaRows * a.head_dim;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (ka.few_rows) {
