@@ -62,7 +62,7 @@ constexpr uint32_t kBlockCols = 256, kOCol = 128;
 constexpr int kFmaEvery = KFMA;
 constexpr int kMinRun = 4;    // cost a run holds at least (its cache tiles and one for each row tile)
 constexpr int kSnapTiles = 8;  // row tiles of up to so many cache tiles are not cut
-constexpr int kGroups = 36;    // groups of requests whose costs are summed up side by side
+constexpr int kGroups = 64;    // groups of requests whose costs are summed up side by side
 
 template <int kDim>
 constexpr size_t tc_smem() {
@@ -142,6 +142,7 @@ struct Place {
 // What the requests of [b0, b1) cost under one KV head (a warp).
 __device__ long long requests_cost(const ChunkArgs& ka, int b0, int b1) {
   const int lane = threadIdx.x & 31;
+  if (b0 >= b1) return 0;
   long long sum = 0;
   for (int c0 = b0; c0 < b1; c0 += 32) {
     const Request mine = c0 + lane < b1 ? read_request(ka.a, c0 + lane, false) : Request{};
@@ -163,12 +164,25 @@ __device__ long long requests_cost(const ChunkArgs& ka, int b0, int b1) {
 // finds the same.
 __device__ Place locate(const ChunkArgs& ka, long long g, const long long* group_cost, int group_size) {
   const int lane = threadIdx.x & 31, H = ka.a.num_kv_heads;
-  int grp = 0;
-  while (grp < kGroups && g >= group_cost[grp] * H) g -= group_cost[grp++] * H;
+  // the group: kGroups <= 64, two per lane
+  const long long c0 = group_cost[2 * lane], c1 = group_cost[2 * lane + 1];
+  long long incl = c0 + c1;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += o;
+  }
   Place at{ka.a.batch, 0, 0, 0};
-  if (grp == kGroups) return at;
+  const uint32_t hits = __ballot_sync(0xffffffffu, incl * H > g);
+  if (!hits) return at;
+  const int src = __ffs(hits) - 1;
+  long long before = incl - c0 - c1;
+  const bool second = (before + c0) * H <= g;
+  if (second) before += c0;
+  g -= __shfl_sync(0xffffffffu, before, src) * H;
+  const int grp = 2 * src + __shfl_sync(0xffffffffu, (int)second, src);
   for (int b = grp * group_size; b < min((grp + 1) * group_size, ka.a.batch); ++b) {
-    const long long cost = requests_cost(ka, b, b + 1);
+    const long long cost = group_size == 1 ? group_cost[grp] : requests_cost(ka, b, b + 1);
     if (g >= cost * H) {
       g -= cost * H;
       continue;
@@ -328,8 +342,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     for (int k = 0; k < 8; ++k) s_move[k] = 0xffffffffu;
   }
   __syncthreads();
-  long long total = 0;
-  for (int g = 0; g < kGroups; ++g) total += s_words.cost[g];
+  long long total = s_words.cost[lane] + s_words.cost[lane + 32];
+#pragma unroll
+  for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
   total *= a.num_kv_heads;
   const int runs = (int)max(1LL, min((long long)gridDim.x, total / kMinRun));
   int4* record = ka.runs + run;
@@ -908,8 +923,8 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkArgs ka) {
   while (c0 > 0 && ka.runs[c0].w == 1) --c0;  // runs that lie inside the row tile
   const Request rq = read_request(a, rec.x, false);
   constexpr int kPer = kDim / 32;
-  for (int r = (int)blockIdx.y * 4 + warp; r < kCtaRows; r += 4 * (int)gridDim.y) {
-    const int row = rec.z * kCtaRows + r;
+  {
+    const int r = (int)blockIdx.y * 4 + warp, row = rec.z * kCtaRows + r;
     if (row >= rq.n * G) return;
     const int tok = row / G, head = rec.y * G + row - tok * G, t = rq.q0 + tok, pos = rq.first_pos + tok;
     auto part = [&](int c) { return ((size_t)2 * c + (c == c0 ? 1 : 0)) * kCtaRows + r; };
@@ -950,7 +965,7 @@ __global__ void __launch_bounds__(128) chunk_merge_kernel(const ChunkArgs ka) {
     }
     if (__any_sync(0xffffffffu, odd) && lsum == lsum && pos >= 0) {  // see the epilogue above
       attn_row<kHalf, kDim>(ka, rec.x, pos, t, head);
-      continue;
+      return;
     }
     uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + (size_t)t * a.o_token_stride +
                                                 (size_t)head * a.o_head_stride);
@@ -1057,7 +1072,7 @@ static int launch_chunk(ChunkArgs& ka, cudaStream_t stream) {
   chunk_attn_tc_kernel<kHalf, kDim><<<ka.ctas, kChunkThreads, tc_smem<kDim>(), stream>>>(ka, tmap_k, tmap_v);
   const int launched = cuda_check(cudaGetLastError());
   if (launched) return launched;
-  return launch_dependent(chunk_merge_kernel<kHalf, kDim>, dim3((unsigned)ka.ctas, 16), dim3(128), 0, stream, ka);
+  return launch_dependent(chunk_merge_kernel<kHalf, kDim>, dim3((unsigned)ka.ctas, kCtaRows / 4), dim3(128), 0, stream, ka);
 }
 
 extern "C" int subspec_chunk_attention_paged(const subspec_chunk_attn_args* args, subspec_stream_t stream) {

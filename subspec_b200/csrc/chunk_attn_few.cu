@@ -446,26 +446,29 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   }
 }
 
-// Joins the (request, KV head)s that lie in several runs: a CTA per (run that holds the end of one, row).
-template <bool kHalf, int kDim, int kMT>
+// Joins the (request, KV head)s that lie in several runs: a warp per (run that holds the end of one, row).
+template <bool kHalf, int kDim>
 __global__ void __launch_bounds__(128) chunk_few_join_kernel(const ChunkArgs ka) {
-  __shared__ float s_acc[128][9];
   const subspec_chunk_attn_args& a = ka.a;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = ka.group, grow = (int)blockIdx.y;
+  const int lane = threadIdx.x & 31, G = ka.group, grow = (int)(blockIdx.y * 4 + (threadIdx.x >> 5));
   grid_dep_wait();
   const int4 rec = ka.few_runs[blockIdx.x];
   if (rec.w != 3) return;
   const int c1 = (int)blockIdx.x;
-  int c0 = c1 - 1;
-  while (c0 > 0 && ka.few_runs[c0].w == 1) --c0;  // runs that lie inside it
+  int c0 = c1;
+  for (bool more = true; more;) {  // back over the runs that lie inside it, 32 at a time, to the one where it begins
+    const int c = c0 - 1 - lane;
+    const uint32_t stop = __ballot_sync(0xffffffffu, c <= 0 || ka.few_runs[c].w != 1);
+    more = stop == 0;
+    c0 -= more ? 32 : __ffs(stop);
+  }
   const int b = rec.x;
   const Request rq = read_request(a, b, false);
-  const int i = grow / G, t = rq.q0 + i, head = rec.y * G + grow - i * G;
+  const int i = grow / G, t = rq.q0 + i, head = rec.y * G + grow - i * G, pos = rq.first_pos + i;
   if (i >= rq.n) return;
-  constexpr int kChunks = kDim / 8, kGroups = 128 / kChunks;
-  const int ch = (int)threadIdx.x % kChunks, grp = (int)threadIdx.x / kChunks;
-  auto row_of = [&](int c) { return ((size_t)2 * c + (c == c0 ? 1 : 0)) * (16 * kMT) + grow; };
-  float mstar = -INFINITY, lsum = 0.f, acc[8] = {};
+  constexpr int kPer = kDim / 32;
+  auto row_of = [&](int c) { return ((size_t)2 * c + (c == c0 ? 1 : 0)) * ka.few_rows + grow; };
+  float mstar = -INFINITY;
   for (int c = c0 + lane; c <= c1; c += 32) {
     const float2 ml = reinterpret_cast<const float2*>(ka.few_ml)[row_of(c)];
     if (ml.y != 0.f) mstar = max3_nan(mstar, ml.x, ml.x);
@@ -475,48 +478,36 @@ __global__ void __launch_bounds__(128) chunk_few_join_kernel(const ChunkArgs ka)
     const float y = __shfl_xor_sync(0xffffffffu, mstar, d);
     mstar = max3_nan(mstar, y, y);
   }
-#pragma unroll 4
-  for (int c = c0 + grp; c <= c1; c += kGroups) {
+  float acc[kPer] = {}, lsum = 0.f;
+#pragma unroll 8
+  for (int c = c0; c <= c1; ++c) {
     const size_t r = row_of(c);
     const float2 ml = reinterpret_cast<const float2*>(ka.few_ml)[r];
-    const float4* src = reinterpret_cast<const float4*>(ka.few_o + r * kDim) + 2 * ch;
-    const float4 x = src[0], y = src[1];
-    if (ml.y == 0.f) continue;  // nothing seen in this part
-    const float w = ex2f(ml.x - mstar);
-    lsum += w * ml.y;
-    acc[0] += w * x.x, acc[1] += w * x.y, acc[2] += w * x.z, acc[3] += w * x.w;
-    acc[4] += w * y.x, acc[5] += w * y.y, acc[6] += w * y.z, acc[7] += w * y.w;
+    float o[kPer];
+    if (kPer == 4)
+      *reinterpret_cast<float4*>(o) = reinterpret_cast<const float4*>(ka.few_o + r * kDim)[lane];
+    else
+      *reinterpret_cast<float2*>(o) = reinterpret_cast<const float2*>(ka.few_o + r * kDim)[lane];
+    const float w = ml.y == 0.f ? 0.f : ex2f(ml.x - mstar);  // (0: nothing seen in this part)
+    lsum += w == 0.f ? 0.f : w * ml.y;
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) acc[x] += w == 0.f ? 0.f : w * o[x];
   }
+  const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
+  bool odd = lsum == 0.f;
 #pragma unroll
-  for (int x = 0; x < 8; ++x) s_acc[threadIdx.x][x] = acc[x];
-  s_acc[threadIdx.x][8] = lsum;
-  __syncthreads();
-  if (warp > 0) return;
-  const int pos = rq.first_pos + i;
-  bool odd = false;
-  if (lane < kChunks) {
-#pragma unroll
-    for (int x = 0; x < 8; ++x) acc[x] = 0.f;
-    lsum = 0.f;
-    for (int k = 0; k < kGroups; ++k) {
-      const float* src = s_acc[k * kChunks + lane];
-#pragma unroll
-      for (int x = 0; x < 8; ++x) acc[x] += src[x];
-      lsum += src[8];
-    }
-    const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
-    odd = lsum == 0.f;
-#pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      acc[x] *= inv;
-      odd = odd || !(fabsf(acc[x]) < INFINITY);
-    }
-    odd = odd && lsum == lsum && pos >= 0;
-    const uint4 v = make_uint4(pack16<kHalf>(acc[0], acc[1]), pack16<kHalf>(acc[2], acc[3]), pack16<kHalf>(acc[4], acc[5]),
-                               pack16<kHalf>(acc[6], acc[7]));
-    reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + (size_t)t * a.o_token_stride + (size_t)head * a.o_head_stride)[lane] = v;
+  for (int x = 0; x < kPer; ++x) {
+    acc[x] *= inv;
+    odd = odd || !(fabsf(acc[x]) < INFINITY);
   }
-  if (__any_sync(0xffffffffu, odd)) attn_row<kHalf, kDim>(ka, b, pos, t, head);
+  if (__any_sync(0xffffffffu, odd) && lsum == lsum && pos >= 0) {
+    attn_row<kHalf, kDim>(ka, b, pos, t, head);
+    return;
+  }
+  uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.out) + (size_t)t * a.o_token_stride +
+                                              (size_t)head * a.o_head_stride);
+#pragma unroll
+  for (int x = 0; x < kPer / 2; ++x) out[lane * (kPer / 2) + x] = pack16<kHalf>(acc[2 * x], acc[2 * x + 1]);
 }
 
 template <bool kHalf, int kDim, int kMT>
@@ -529,7 +520,7 @@ int launch(ChunkArgs& ka, cudaStream_t stream) {
   const int launched = cuda_check(cudaGetLastError());
   if (launched) return launched;
   const long long rows = (long long)ka.a.max_q_len * ka.group;
-  return launch_dependent(chunk_few_join_kernel<kHalf, kDim, kMT>, dim3(kFewCtas, (unsigned)(rows < 16 * kMT ? rows : 16 * kMT)),
+  return launch_dependent(chunk_few_join_kernel<kHalf, kDim>, dim3(kFewCtas, (unsigned)((rows < 16 * kMT ? rows : 16 * kMT) + 3) / 4),
                           dim3(128), 0, stream, ka);
 }
 
