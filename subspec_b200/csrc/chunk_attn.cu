@@ -61,7 +61,7 @@ constexpr uint32_t kBlockCols = 256, kOCol = 128;
 #endif
 constexpr int kFmaEvery = KFMA;
 constexpr int kMinRun = 4;    // cost a run holds at least (its cache tiles and one for each row tile)
-constexpr int kSnapTiles = 8;  // row tiles of up to so many cache tiles are not cut
+constexpr int kSnapTiles = 8;  // row tiles of up to so many cache tiles are not cut where runs are long
 constexpr int kGroups = 64;    // groups of requests whose costs are summed up side by side
 
 template <int kDim>
@@ -124,7 +124,7 @@ struct RowTile {
   __device__ __forceinline__ RowTile(const ChunkArgs& ka, const Request& rq, int qt)
       : row0(qt * kCtaRows),
         rows(rq.n * ka.group),
-        list(rq.first_pos + row0 / ka.group, rq.first_pos + (min(row0 + kCtaRows, rows) - 1) / ka.group, ka.a.window, ka.a.sinks) {
+        list(rq.first_pos + by_group(ka, row0), rq.first_pos + by_group(ka, min(row0 + kCtaRows, rows) - 1), ka.a.window, ka.a.sinks) {
     n = max(list.n, 1);
   }
   __device__ __forceinline__ int cost() const { return n + 1; }
@@ -162,7 +162,7 @@ __device__ long long requests_cost(const ChunkArgs& ka, int b0, int b1) {
 
 // The place `g` into the line (a warp).  Places inside short row tiles, or next to an edge, move to the edge: every CTA
 // finds the same.
-__device__ Place locate(const ChunkArgs& ka, long long g, const long long* group_cost, int group_size) {
+__device__ Place locate(const ChunkArgs& ka, long long g, const long long* group_cost, int group_size, int snap) {
   const int lane = threadIdx.x & 31, H = ka.a.num_kv_heads;
   // the group: kGroups <= 64, two per lane
   const long long c0 = group_cost[2 * lane], c1 = group_cost[2 * lane + 1];
@@ -207,7 +207,7 @@ __device__ Place locate(const ChunkArgs& ka, long long g, const long long* group
         at.qt = q0 + src;
         const int n = __shfl_sync(0xffffffffu, tile.n, src);
         at.i = (int)(g - __shfl_sync(0xffffffffu, incl - own, src));
-        if (n <= kSnapTiles)
+        if (n <= snap)
           at.i = 2 * at.i < n ? 0 : n;
         else if (at.i < 2 || at.i > n - 2)
           at.i = at.i < 2 ? 0 : n;
@@ -347,6 +347,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
   total *= a.num_kv_heads;
   const int runs = (int)max(1LL, min((long long)gridDim.x, total / kMinRun));
+  // row tiles of up to so many cache tiles are not cut: a part costs about two tiles, an uneven run up to half the tile
+  const int snap = (int)min((long long)kSnapTiles, total / runs / 4);
   int4* record = ka.runs + run;
   if (total == 0 || run >= runs) {
     if (warp == 0) report();
@@ -355,7 +357,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   }
   if (warp < 2) {
     const int c = run + warp;
-    const Place p = c < runs ? locate(ka, c * total / runs, s_words.cost, group_size) : Place{a.batch, 0, 0, 0};
+    const Place p = c < runs ? locate(ka, c * total / runs, s_words.cost, group_size, snap) : Place{a.batch, 0, 0, 0};
     if (lane == 0) s_place[warp] = p;
   }
   if (warp == kIssuerWarp) {
@@ -383,8 +385,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   // Rows of a block of a piece: cache rows of its first and last token; a block without rows sees nothing.
   auto block_pos = [&](const Piece& pc, int blk, int& first, int& last) {
     const int r0 = pc.row0 + blk * kBlockRows;
-    first = pc.first_pos + r0 / G;
-    last = r0 < pc.rows ? pc.first_pos + (min(r0 + kBlockRows, pc.rows) - 1) / G : -1;
+    first = pc.first_pos + by_group(ka, r0);
+    last = r0 < pc.rows ? pc.first_pos + by_group(ka, min(r0 + kBlockRows, pc.rows) - 1) : -1;
   };
   // Whether a block's rows see anything of tile row t0, and whether all of them see all of it.
   auto block_sees = [&](int first, int last, int t0) {
@@ -428,7 +430,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     auto load_q = [&](const Piece& pc) {
       constexpr int kChunks = kDim / 8, kPass = 32 / kChunks;  // chunks of a row, rows at once
       const int c = lane % kChunks, r0 = (warp & 7) * 16 + lane / kChunks;
-      int row = pc.row0 + blk * kBlockRows + r0, tok = row / G, g = row - tok * G;
+      int row = pc.row0 + blk * kBlockRows + r0, tok = by_group(ka, row), g = row - tok * G;
       unsigned char* d = qtiles + blk * kQBlockBytes + (c >> 3) * kQHalfBytes;
 #pragma unroll
       for (int x = 0; x < 16; x += kPass) {
@@ -461,7 +463,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if (pair_or(pair, now == nullptr)) break;  // (both or neither: they meet at barriers)
       const int row = now->row0 + blk * kBlockRows + rr;
       const bool row_ok = row < now->rows, block_ok = now->row0 + blk * kBlockRows < now->rows, whole = now->whole;
-      const int tok = row / G, head = now->h * G + row - tok * G, t = now->q0 + tok, b = now->b;
+      const int tok = by_group(ka, row), head = now->h * G + row - tok * G, t = now->q0 + tok, b = now->b;
       int bfirst, blast;
       block_pos(*now, blk, bfirst, blast);
       const int pos = min(now->first_pos + tok, blast);  // rows that do not exist look like the last one
@@ -1002,6 +1004,12 @@ static void chunk_sizes(ChunkArgs& ka) {
   const long long most = (long long)a.max_q_len * ka.group;
   const long long others = (long long)(a.tokens - a.max_q_len) * ka.group;
   ka.few_rows = most <= 16 ? 16 : most <= 32 ? 32 : a.batch > 1 && others <= 64LL * (a.batch - 1) ? 16 : 0;
+  if (ka.group > 1) {
+    int l = 0;
+    while ((1LL << l) < ka.group) ++l;
+    ka.group_mul = (uint32_t)(((1ULL << (31 + l)) + ka.group - 1) / ka.group);
+    ka.group_shift = (uint32_t)(l - 1);
+  }
   if (ka.few_rows >= most) {
     ka.ctas = 0;
     return;
