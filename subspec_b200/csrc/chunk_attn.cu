@@ -56,10 +56,7 @@ constexpr int kSoftmaxWarps = 16;
 constexpr int kChunkThreads = 32 * (kSoftmaxWarps + 4);
 constexpr int kIssuerWarp = kSoftmaxWarps, kLoadWarp = kIssuerWarp + 2;
 constexpr uint32_t kBlockCols = 256, kOCol = 128;
-#ifndef KFMA
-#define KFMA 8
-#endif
-constexpr int kFmaEvery = KFMA;
+constexpr int kFmaEvery = 8;   // of the pairs of exponentials one in so many goes to the FMA pipe (3, 4, 16: within 2 %)
 constexpr int kMinRun = 4;    // cost a run holds at least (its cache tiles and one for each row tile)
 constexpr int kSnapTiles = 8;  // row tiles of up to so many cache tiles are not cut where runs are long
 constexpr int kGroups = 64;    // groups of requests whose costs are summed up side by side
@@ -353,6 +350,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   if (total == 0 || run >= runs) {
     if (warp == 0) report();
     if (threadIdx.x == 0) *record = make_int4(0, 0, 0, 0);
+    grid_dep_wait();
     return;
   }
   if (warp < 2) {
@@ -908,6 +906,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  // (Launched behind the kernel for few rows it begins as that one's blocks leave, and needs nothing from it; but whoever
+  // waits for this kernel waits for that one, too.)
+  grid_dep_wait();
 }
 
 // Joins the row tiles that were cut: the run that holds a tile's end (blockIdx.x) adds up the runs' unnormalised rows, a
@@ -1077,8 +1078,14 @@ static int launch_chunk(ChunkArgs& ka, cudaStream_t stream) {
   if (rc) return rc;
   CUtensorMap tmap_k, tmap_v;
   chunk_tensor_maps(ka, kTileKeys, &tmap_k, &tmap_v);
-  chunk_attn_tc_kernel<kHalf, kDim><<<ka.ctas, kChunkThreads, tc_smem<kDim>(), stream>>>(ka, tmap_k, tmap_v);
-  const int launched = cuda_check(cudaGetLastError());
+  int launched;
+  if (ka.few_rows) {
+    launched = launch_dependent(chunk_attn_tc_kernel<kHalf, kDim>, dim3((unsigned)ka.ctas), dim3(kChunkThreads), tc_smem<kDim>(),
+                                stream, ka, tmap_k, tmap_v);
+  } else {
+    chunk_attn_tc_kernel<kHalf, kDim><<<ka.ctas, kChunkThreads, tc_smem<kDim>(), stream>>>(ka, tmap_k, tmap_v);
+    launched = cuda_check(cudaGetLastError());
+  }
   if (launched) return launched;
   return launch_dependent(chunk_merge_kernel<kHalf, kDim>, dim3((unsigned)ka.ctas, kCtaRows / 4), dim3(128), 0, stream, ka);
 }

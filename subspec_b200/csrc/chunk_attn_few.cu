@@ -2,7 +2,7 @@
 // computed on it (2 * rows flop a byte: HBM-bound up to hundreds of rows).
 //
 // The work of the call is one line of cache tiles -- requests, their KV heads, their tiles of 64 cache rows one behind
-// the other -- cut into equal runs, one per CTA (two CTAs an SM): ragged batches and lone long caches load every SM
+// the other -- cut into equal runs, one per CTA (three CTAs an SM, so that the ends of one's pieces lie under the others' copies): ragged batches and lone long caches load every SM
 // alike.  A run is walked in pieces, a piece being what it has of one (request, head).  Each of the CTA's four warps
 // takes 16 of a tile's 64 rows and works on its own: it has a ring of stages (16 K and 16 V rows each) that its lanes
 // fill by tensor copies, and computes, with Q in registers as the A operand of m16n8k16,
@@ -22,11 +22,12 @@ namespace {
 constexpr int kFewWarps = 4, kFewThreads = 32 * kFewWarps;
 constexpr int kWarpKeys = 16;
 constexpr int kFewTile = kFewWarps * kWarpKeys;
-constexpr int kFewCtas = 2 * kNumSMs;
+constexpr int kFewPerSm = 3;
+constexpr int kFewCtas = kFewPerSm * kNumSMs;
 constexpr int kFewMinTiles = 4;  // tiles a run holds at least: a part costs as much to join as a tile to read
 
 template <int kDim>
-constexpr int few_stages() { return 384 / kDim; }  // 24 KB a warp
+constexpr int few_stages() { return 256 / kDim; }  // 16 KB a warp
 template <int kDim>
 constexpr int few_stage_bytes() { return 2 * kWarpKeys * kDim * 2; }
 template <int kDim>
@@ -84,7 +85,7 @@ struct Cursor {
 };
 
 template <bool kHalf, int kDim, int kMT>
-__global__ void __launch_bounds__(kFewThreads, 2)
+__global__ void __launch_bounds__(kFewThreads, kFewPerSm)
     chunk_attn_few_kernel(const ChunkArgs ka, const __grid_constant__ CUtensorMap tmap_k,
                           const __grid_constant__ CUtensorMap tmap_v) {
   extern __shared__ unsigned char smem_raw[];
@@ -451,6 +452,7 @@ template <bool kHalf, int kDim>
 __global__ void __launch_bounds__(128) chunk_few_join_kernel(const ChunkArgs ka) {
   const subspec_chunk_attn_args& a = ka.a;
   const int lane = threadIdx.x & 31, G = ka.group, grow = (int)(blockIdx.y * 4 + (threadIdx.x >> 5));
+  grid_dep_launch();  // (the kernel for many rows needs nothing of this one's)
   grid_dep_wait();
   const int4 rec = ka.few_runs[blockIdx.x];
   if (rec.w != 3) return;

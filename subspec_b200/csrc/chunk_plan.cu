@@ -22,6 +22,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kPlanThreads = 1024;
+static_assert(kPlanThreads == 32 * 32, "the block scan takes a partial sum from each of 32 warps");
 constexpr int kPlanMaxCtas = 8;  // one cluster of the portable size: its barrier orders the phases
 
 // Exclusive scan of two ints per thread over the CTA (carried in one 64-bit word: both sums stay below 2^31).

@@ -362,6 +362,49 @@ def test_scores_of_all_sizes(cuda_lib):
         assert status.item() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("step", [4.0, 30.0, 45.0, 80.0])
+def test_scores_that_rise_by_steps(cuda_lib, dtype, step):
+    """Scores that rise by `step` every 100 rows, and fall again: the reference point of the weights has to follow over
+    many tiles (4: it need not; 30, 45: between the tiles; 80: further than the types' weights reach within one)."""
+    for new, cached in (([1], [900]), ([40], [860])):
+        c = _setup(21, new, cached, 4, 2, dtype=dtype)
+        n = c["kv_len"][0]
+        level = (torch.arange(n) // 100).clamp(max=6) * step
+        level[700:] = 0
+        c["ks"][0] *= 0
+        c["ks"][0][:, :, 0] = (level / 16)[:, None].to(dtype)
+        c["q"] *= 0
+        c["q"][:, :, 0] = 16.0
+        for j in range(n):
+            c["pool"][1, c["table"][0, j // 16], 0, j % 16] = c["ks"][0][j]
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        got = _run(c, status=status, sm_scale=1.0)
+        want, mag = ao.chunk_attention(c["q"], c["ks"][0], c["vs"][0], sm_scale=1.0)
+        # the scores are single products, exact in fp32; scaled to powers of two (up to 480 * 1.44) they are off by 2^-15
+        tol = _tolerance(want, mag, n, dtype, 6.0) + 2 ** -14 * mag
+        assert bool(((got.double().cpu() - want).abs() <= tol).all()) and status.item() == 0
+
+
+def test_values_that_are_not_finite_and_seen(cuda_lib):
+    """NaN and infinite scores and values that a row does see: the row comes out as the formula has it."""
+    for new in ([1, 1], [70, 30]):
+        for plane, bad in ((0, float("nan")), (1, float("nan")), (1, float("inf"))):
+            c = _setup(22, new, [300, 200], 4, 2)
+            for b in range(2):
+                j = 133
+                (c["ks"] if plane == 0 else c["vs"])[b][j, :, 7] = bad
+                c["pool"][1, c["table"][b, j // 16], plane, j % 16, :, 7] = bad
+            got = _run(c).double().cpu()
+            for b, n in enumerate(new):
+                lo = c["indptr"][b]
+                want, mag = ao.chunk_attention(c["q"][lo:lo + n], c["ks"][b], c["vs"][b])
+                g, fine = got[lo:lo + n], torch.isfinite(want)
+                assert torch.equal(torch.isnan(g), torch.isnan(want)) and torch.equal(torch.isfinite(g), fine)
+                tol = _tolerance(want, mag, c["kv_len"][b], torch.bfloat16, 6.0)
+                assert bool(((g - want).abs()[fine] <= tol[fine]).all())
+
+
 def test_layouts_of_q_and_out(cuda_lib):
     """q as a slice of a fused projection, heads in front of tokens, odd addresses; out with strides of its own, its
     padding and the rows behind the last request untouched."""
