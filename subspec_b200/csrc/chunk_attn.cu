@@ -56,7 +56,6 @@ constexpr int kSoftmaxWarps = 16;
 constexpr int kChunkThreads = 32 * (kSoftmaxWarps + 4);
 constexpr int kIssuerWarp = kSoftmaxWarps, kLoadWarp = kIssuerWarp + 2;
 constexpr uint32_t kBlockCols = 256, kOCol = 128;
-constexpr int kFmaEvery = 8;   // of the pairs of exponentials one in so many goes to the FMA pipe (3, 4, 16: within 2 %)
 constexpr int kMinRun = 4;    // cost a run holds at least (its cache tiles and one for each row tile)
 constexpr int kSnapTiles = 8;  // row tiles of up to so many cache tiles are not cut where runs are long
 constexpr int kGroups = 64;    // groups of requests whose costs are summed up side by side
@@ -90,27 +89,6 @@ __device__ __forceinline__ bool pair_or(int id, bool x) {
 
 // First cache row of entry i of a tile list.
 __device__ __forceinline__ int list_row(int s_tiles, int m0, int i) { return (i < s_tiles ? i : m0 + i - s_tiles) * kTileKeys; }
-
-// 2^x for a pair of exponents without the special-function unit: x = n + f with n = round(x), f in [-0.5, 0.5]; 2^f by the
-// cubic of least relative error (1.0e-4, a nineteenth of what rounding a weight to bf16 costs, a fifth for fp16) among
-// those that are 1 at 0 -- so that everything below 2^-127, -inf first of all, becomes 0 exactly -- and n added into the
-// exponent field (the magic constant 1.5 * 2^23 leaves it in the low bits).  A NaN comes out as 3.4e38, which the sums notice.
-__device__ __forceinline__ void exp2_pair(float x0, float x1, float& p0, float& p1) {
-  asm("min.NaN.xorsign.abs.f32 %0, %0, %1;" : "+f"(x0) : "f"(127.f));  // into [-127, 127]
-  asm("min.NaN.xorsign.abs.f32 %0, %0, %1;" : "+f"(x1) : "f"(127.f));
-  const uint64_t x = f2_pack(x0, x1), one = f2_pack(1.f, 1.f);
-  const uint64_t t2 = f2_add(x, f2_pack(12582912.f, 12582912.f));
-  const uint64_t n2 = f2_add(t2, f2_pack(-12582912.f, -12582912.f));
-  const uint64_t f2 = f2_fma(n2, f2_pack(-1.f, -1.f), x);
-  uint64_t q = f2_fma(f2_pack(0.0550090596f, 0.0550090596f), f2, f2_pack(0.242210969f, 0.242210969f));
-  q = f2_fma(q, f2, f2_pack(0.693282902f, 0.693282902f));
-  q = f2_fma(q, f2, one);
-  float q0, q1, t0, t1;
-  f2_unpack(q, q0, q1);
-  f2_unpack(t2, t0, t1);
-  p0 = __int_as_float(__float_as_int(q0) + (__float_as_int(t0) << 23));
-  p1 = __int_as_float(__float_as_int(q1) + (__float_as_int(t1) << 23));
-}
 
 // A row tile: rows [row0, row0 + 256) of the n * group (token, head) rows of a request under one KV head.
 struct RowTile {
@@ -430,7 +408,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const int c = lane % kChunks, r0 = (warp & 7) * 16 + lane / kChunks;
       int row = pc.row0 + blk * kBlockRows + r0, tok = by_group(ka, row), g = row - tok * G;
       unsigned char* d = qtiles + blk * kQBlockBytes + (c >> 3) * kQHalfBytes;
-#pragma unroll
+#pragma unroll 2
       for (int x = 0; x < 16; x += kPass) {
         const int r = r0 + x;
         const bool ok = row < pc.rows;
@@ -542,14 +520,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           auto weights = [&](uint32_t (&r)[32], uint32_t (&pk)[16]) {
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              float x0, x1, p0, p1;
+              float x0, x1;
               f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), c2p, nup), x0, x1);
-              if (j % kFmaEvery == kFmaEvery - 1) {
-                exp2_pair(x0, x1, p0, p1);  // some pairs on the FMA pipe
-              } else {
-                p0 = ex2f(x0);
-                p1 = ex2f(x1);
-              }
+              const float p0 = ex2f(x0), p1 = ex2f(x1);  // 2^-inf = 0: hidden entries get the weight 0 exactly
               sm2[j & 3] = f2_add(sm2[j & 3], f2_pack(p0, p1));
               pk[j] = pack16<kHalf>(p0, p1);
             }
@@ -614,41 +587,35 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                           half * (kDim / 2);
       float* part_row = ka.part_o + prow * kDim + half * (kDim / 2);
       if (!whole && row_ok && half == 0) reinterpret_cast<float2*>(ka.part_ml)[prow] = make_float2(m, l);
+      // (Sixteen columns at a time in a loop: this code runs once a row tile, out of a cold instruction cache.)
+#pragma unroll 1
+      for (int c = 0; c < kDim / 2; c += 16) {
+        uint32_t rc[16];
 #pragma unroll
-      for (int c = 0; c < kDim / 64; ++c) {
-        uint32_t rc[32];
+        for (int j = 0; j < 16; ++j) rc[j] = 0u;
         if (done > 0) {
-          tmem_ld32_async(o_addr + 32 * c, rc);
+          tmem_ld16_async(o_addr + c, rc);
           tmem_wait_ld_dep(rc);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) rc[j] = 0u;
         }
         if (!whole) {
           if (row_ok) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) store32(part_row + 32 * c + 8 * j, &rc[8 * j]);
+            store32(part_row + c, rc);
+            store32(part_row + c + 8, rc + 8);
           }
-        } else {
+          continue;
+        }
+        uint32_t v[8];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float x = pos < 0 ? 0.f : __uint_as_float(rc[j]) * inv;
-            odd = odd || !(fabsf(x) < INFINITY);
-            rc[j] = __float_as_uint(x);
-          }
-          if (row_ok) {
-            uint32_t v[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = pack16<kHalf>(__uint_as_float(rc[2 * j]), __uint_as_float(rc[2 * j + 1]));
-            if (wide_out) {
-              store32(out_row + 32 * c, v);
-              store32(out_row + 32 * c + 16, v + 8);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                reinterpret_cast<uint4*>(out_row)[4 * c + j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            }
-          }
+        for (int j = 0; j < 8; ++j) {
+          const float x = pos < 0 ? 0.f : __uint_as_float(rc[2 * j]) * inv, y = pos < 0 ? 0.f : __uint_as_float(rc[2 * j + 1]) * inv;
+          odd = odd || !(fabsf(x) < INFINITY) || !(fabsf(y) < INFINITY);
+          v[j] = pack16<kHalf>(x, y);
+        }
+        if (row_ok && wide_out) {
+          store32(out_row + c, v);
+        } else if (row_ok) {
+          reinterpret_cast<uint4*>(out_row + c)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+          reinterpret_cast<uint4*>(out_row + c)[1] = make_uint4(v[4], v[5], v[6], v[7]);
         }
       }
       tc_fence_before();
