@@ -322,6 +322,8 @@ def on_device(fn, args, device, what: str) -> None:
     """Call an entry point on `device`'s current stream, with `device` current for its launches."""
     import torch
 
+    if device.type != "cuda":
+        raise ValueError(f"{what}: the tensors must be on a CUDA device, there is no CPU form")
     index = device.index
     if index == torch.cuda.current_device():
         check(fn(C.byref(args), _raw_stream(index)), what)

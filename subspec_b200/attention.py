@@ -240,8 +240,16 @@ def append_paged_kv_slots(pool: torch.Tensor, layer: int, k: torch.Tensor, v: to
         v = v.detach().clone(memory_format=torch.contiguous_format)
     a = _lib.KvAppendSlotsArgs(C.sizeof(_lib.KvAppendSlotsArgs), T, H, D, layer, L, P, page_len, pool.data_ptr(),
                                k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                               slot_map.data_ptr(), 0 if status is None else status.data_ptr())
+                               slot_map.data_ptr(), _status_ptr(status, dev))
     _lib.on_device(_lib.lib().subspec_kv_append_slots, a, dev, "subspec_kv_append_slots")
+
+
+def _status_ptr(status: Optional[torch.Tensor], dev) -> int:
+    if status is None:
+        return 0
+    if status.dtype != torch.int32 or status.device != dev or status.numel() < 1:
+        raise ValueError("status must be an int32 tensor on the pool's device")
+    return status.data_ptr()
 
 
 @functools.lru_cache(maxsize=1024)
@@ -271,6 +279,8 @@ def _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, wi
         out = torch.empty(T, HQ, D, dtype=q.dtype, device=dev)
     elif out.dtype != q.dtype or out.shape != shape or out.device != dev or not (T == 0 or _aligned(out)):
         raise ValueError("out must be a tensor of q's type and shape on q's device, its rows 16-byte aligned")
+    elif T and out.data_ptr() == q.data_ptr():
+        raise ValueError("out must not be q itself")
     max_q_len = T if max_q_len is None else int(max_q_len)
     if max_q_len < 0:
         raise ValueError("max_q_len must not be negative")
@@ -286,7 +296,7 @@ def _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, wi
                            _lib.BF16 if q.dtype == torch.bfloat16 else _lib.F16, window, sinks, 0,
                            pool.data_ptr(), page_table.data_ptr(), kv_ptr, indptr_ptr, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
                            1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
-                           0 if status is None else status.data_ptr(), 0 if scratch is None else scratch.data_ptr(), need)
+                           _status_ptr(status, dev), 0 if scratch is None else scratch.data_ptr(), need)
     _lib.on_device(_lib.lib().subspec_chunk_attention_paged, a, dev, "subspec_chunk_attention_paged")
     return out  # (torch's allocator keeps the scratch for this stream until the kernels have passed)
 
@@ -302,7 +312,8 @@ def chunk_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, pa
     (append first), and each sees the rows up to its own.  One token (a decode step) to whole prompts, mixed at will.
     `max_q_len`: no request brings more (default: all the tokens) -- give it where it is known, the kernels for a few
     rows per request are chosen by it.  Rows of the output behind q_indptr[-1] are left as they were; what a token does
-    not see has no influence on it, infinities and NaN included.  What `DevicePagePool.plan_chunks` returned fits as
+    not see has no influence on it, infinities and NaN included.  `out` must not overlap q.  Requests may share pages
+    (a common prefix).  What `DevicePagePool.plan_chunks` returned fits as
     it is: chunk_attention_paged(q, pool, layer, page_table=plan.page_table, kv_len=plan.kv_len, q_indptr=plan.q_indptr)."""
     return _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, 0, 0, sm_scale, status, out)
 

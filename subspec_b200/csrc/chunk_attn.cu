@@ -30,17 +30,24 @@ namespace {
 // of neighbouring tokens: their KV head's cache rows are read once for the whole group, and the causal border crosses
 // few tiles.  A row tile = 256 rows of one (request, KV head), two blocks that share every K / V tile of 128 cache rows:
 //
-//   warps 0-7   softmax, four warps per block: thread = query row = lane of tensor memory.  Per tile a thread reads its
-//               128 scores and writes P = 2^(S c - m) as 16-bit pairs over the first half of the columns it read,
-//               summing P in fp32.  m, the reference point, is the maximum of the first tile, and moves (the row of O in
-//               tensor memory is rescaled) only when the sums say that a later score has run far ahead of it.  They also
-//               bring the row's Q.
-//   warps 8, 9  issue the MMAs of a block each, in turns: O += P V (P from tensor memory, V MN-major as the cache has
-//               it), in two halves of 64 cache rows as their P comes, then S = Q K^T of the next tile (128 x 128 x
-//               head_dim, both K-major in shared memory) over the P just consumed: the MMAs of a thread run in order.
-//               While one block is in its softmax the other's MMAs run.
-//   warp 10     brings the K tiles, warp 11 the V tiles, into a ring of five entries, K(0), V(0), K(1), V(1), ...;
-//               warp 10 also walks the run and hands out its pieces.
+//   warps 0-15  softmax, eight warps per block: thread = query row = lane of tensor memory, two warps per row, one for
+//               either half of a tile's 128 scores.  A thread writes P = 2^(S c - m) as 16-bit pairs over the first of the
+//               columns it read and sums P in fp32.  m, the reference point, is the maximum of the first tile, and moves
+//               (the row of O in tensor memory is rescaled) only when the sums say that a later score has run far ahead of
+//               it.  They also bring the block's Q and write its output.
+//   warps 16, 17  issue the MMAs of a block each, in turns: O += P V (P from tensor memory, V MN-major as the cache has
+//               it), then S = Q K^T of the next tile (128 x 128 x head_dim, both K-major in shared memory) over the P just
+//               consumed: the MMAs of a thread run in order.  While one block is in its softmax the other's MMAs run.
+//   warp 18     brings the K tiles, warp 19 the V tiles, into a ring of five entries, K(0), V(0), K(1), V(1), ...;
+//               warp 18 also walks the run and hands out its pieces.
+//
+// What it measured (B200, bf16, 28 query heads on 4 KV heads of 128 dims): 2048 tokens behind 30720 rows 745 us =
+// 1251 TFLOP/s, 0.75 of the card's cuBLAS burst (1.08 PFLOP/s at the 1 kW power cap when it runs for seconds).  A tile takes
+// 2058 cycles of MMAs for both blocks and about 3600 in all.  Steps on the way, same case: an issuer per block without
+// turns 1306 us (both blocks in their softmax at once); one issuer 1015; runs over all SMs instead of a CTA per row tile,
+// half a tile of scores in registers instead of spilling, turns 790; two warps per row 756; Q rows by neighbouring lanes
+// and 32-byte stores 745.  Tried and no faster: separate score buffers for the tile's halves (S of 64 columns: MMAs 2484
+// cycles a tile) 740 to 850; a share of the exponentials as a polynomial on the FMA pipe 737 to 760.
 //
 // A tile lies in shared memory as 16 groups of 8 rows; a group as one (head_dim 64) or two halves of 64 dims, a half as
 // 8 rows of 128 bytes under the 128-byte swizzle: the layout the tensor cores read either way round, in which the rows
@@ -202,7 +209,7 @@ __device__ Place locate(const ChunkArgs& ka, long long g, const long long* group
   return at;
 }
 
-// A piece: what a run has of one row tile.  Warp 10 walks the run and hands the pieces to the other warps through shared
+// A piece: what a run has of one row tile.  Warp 18 walks the run and hands the pieces to the other warps through shared
 // memory (a walker of thirty words in every warp pushes the softmax's scores out of the registers).
 struct Piece {
   int valid;                    // 0: the run is over
@@ -749,7 +756,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         mbar_wait_bounded(&drained[blk], 0);
       }
     } else {
-      // ================= K (warp 10) and V (warp 11) tiles =================
+      // ================= K (warp 18) and V (warp 19) tiles =================
       const int is_v = warp - kLoadWarp;
       const CUtensorMap* map = is_v ? &tmap_v : &tmap_k;
       const int box = ka.box_rows, boxes = box > 0 ? kTileKeys / box : 0;
@@ -768,7 +775,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (!p) break;
           now = *p;
           pop();
-        } else {  // warp 10 walks the run and hands out its pieces
+        } else {  // warp 18 walks the run and hands out its pieces
           const bool any = walk.next(ka);
           now = walk.piece(any);
           if (!(live = tc_wait(&pc_empty[pc_slot], slot_ph, abort_flag))) break;
@@ -1069,6 +1076,10 @@ extern "C" int subspec_chunk_attention_paged(const subspec_chunk_attn_args* args
     return SUBSPEC_EUNSUPPORTED;
   ChunkArgs ka{};
   ka.a = a;
+  // beyond the capacity of a request's pages they say nothing more (and sums with them stay within 32 bits)
+  const int cap = a.pages_per_seq * a.page_len;
+  if (ka.a.window > cap) ka.a.window = cap;
+  if (ka.a.sinks > cap) ka.a.sinks = cap;
   chunk_sizes(ka);
   ka.scale_log2 = (float)(a.sm_scale * 1.4426950408889634);
   ka.page_shift = -1;

@@ -275,6 +275,7 @@ extern "C" int subspec_chunk_plan(const subspec_chunk_plan_args* args, subspec_s
   if (!args || args->struct_size != sizeof(subspec_chunk_plan_args)) return SUBSPEC_EINVAL;
   const subspec_chunk_plan_args& a = *args;
   if (a.batch < 0 || a.num_pages < 1 || a.page_len < 1 || a.pages_per_seq < 1 || a.max_tokens < 0) return SUBSPEC_EINVAL;
+  if (a.batch == 0) return SUBSPEC_OK;
   if (!a.free_mask || !a.page_table || !a.n_pages || !a.kv_len || !a.n_new || !a.q_indptr) return SUBSPEC_EINVAL;
   if (a.max_tokens > 0 && (!a.slot_map || !a.positions || !a.batch_indices)) return SUBSPEC_EINVAL;
   // positions, token counts and ranks are 32-bit

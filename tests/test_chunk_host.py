@@ -41,7 +41,7 @@ def _call(fn=chunk_attention_paged, **kw):
     dict(q_indptr=_i32(0, 2)), dict(q_indptr=torch.tensor([0, 2, 3])),
     dict(out=torch.zeros(3, 4, 64)), dict(out=torch.zeros(2, 4, 64, dtype=torch.bfloat16)),
     dict(out=torch.zeros(3, 4, 65, dtype=torch.bfloat16)[..., 1:]),          # rows not 16-byte aligned
-    dict(max_q_len=-1),
+    dict(max_q_len=-1), dict(status=torch.zeros(1, dtype=torch.int64)),
 ])
 def test_attention_refusals(bad):
     with pytest.raises(ValueError):
@@ -75,6 +75,16 @@ def test_plan_refusals():
     for bad in (dict(n_new=_i32(1)), dict(n_new=torch.tensor([1.0, 2.0])), dict(n_new=_i32(1, 1), set_len=_i32(1, 2, 3))):
         with pytest.raises(ValueError):
             pool.plan_chunks(bad["n_new"], set_len=bad.get("set_len"))
+
+
+def test_host_tensors_are_refused(cuda_lib):
+    """There is no CPU form: calls that are right in all else, on host tensors."""
+    for call in (lambda: _call(), lambda: _call(window_attention_paged, window=3),
+                 lambda: append_paged_kv_slots(_pool(), 0, torch.zeros(3, 2, 64, dtype=torch.bfloat16),
+                                               torch.zeros(3, 2, 64, dtype=torch.bfloat16), slot_map=torch.arange(3)),
+                 lambda: DevicePagePool(2, 8, 4, 4, "cpu", max_append=8).plan_chunks(_i32(1, 1))):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
 
 
 def test_c_entry_points_check_their_arguments(cuda_lib):
