@@ -318,28 +318,36 @@ def check(rc: int, what: str) -> None:
     raise SubspecError(f"{what}: {msg}")
 
 
-def on_device(fn, args, device, what: str) -> None:
-    """Call an entry point on `device`'s current stream, with `device` current for its launches."""
-    import torch
-
-    if device.type != "cuda":
+def on_device(fn, args, index: int, what: str) -> None:
+    """Call an entry point on the current stream of device `index` (`Tensor.get_device()`: -1 is the host), with that
+    device current for its launches."""
+    if index < 0:
         raise ValueError(f"{what}: the tensors must be on a CUDA device, there is no CPU form")
-    index = device.index
-    if index == torch.cuda.current_device():
-        check(fn(C.byref(args), _raw_stream(index)), what)
+    if _current_device is None:
+        _torch_handles()
+    if index == _current_device():
+        rc = fn(C.byref(args), _raw_stream(index))
     else:
+        import torch
+
         with torch.cuda.device(index):
-            check(fn(C.byref(args), _raw_stream(index)), what)
+            rc = fn(C.byref(args), _raw_stream(index))
+    if rc:
+        check(rc, what)
 
 
-def _raw_stream(index: int) -> int:
+_current_device = _raw_stream = None
+
+
+def _torch_handles() -> None:
+    """torch.cuda.current_stream builds a Stream object and current_device asks for initialisation each time, 3 us of a
+    small call's 15; torch's own compilers read the handles behind them."""
+    global _current_device, _raw_stream
     import torch
 
-    global _raw_stream
-    # torch.cuda.current_stream builds a Stream object (2 us of a small call's 15); torch's own compilers read the handle
-    get = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    _raw_stream = get or (lambda i: torch.cuda.current_stream(i).cuda_stream)
-    return _raw_stream(index)
+    torch.cuda.init()
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def dev_status_text(word: int) -> str:

@@ -222,12 +222,12 @@ def append_paged_kv_slots(pool: torch.Tensor, layer: int, k: torch.Tensor, v: to
     negative ones are skipped (a padded batch), one past the pool sets `status`.  k and v may be slices of a fused
     projection."""
     L, P, _, page_len, H, D = _check_pool(pool, layer)
-    shape, dev = k.shape, pool.device
-    if len(shape) != 3 or shape != v.shape or shape[1] != H or shape[2] != D or k.dtype != pool.dtype or \
-            v.dtype != pool.dtype or k.device != dev or v.device != dev:
+    shape, dtype, dev = k.shape, pool.dtype, pool.get_device()
+    if len(shape) != 3 or shape != v.shape or shape[1] != H or shape[2] != D or k.dtype != dtype or \
+            v.dtype != dtype or k.get_device() != dev or v.get_device() != dev:
         raise ValueError("k and v must be [tokens, kv_heads, head_dim] tensors of the pool's type on its device")
     T = shape[0]
-    if slot_map.dtype != torch.int64 or slot_map.device != dev or slot_map.dim() != 1 or slot_map.shape[0] < T or \
+    if slot_map.dtype != torch.int64 or slot_map.get_device() != dev or slot_map.dim() != 1 or slot_map.shape[0] < T or \
             not slot_map.is_contiguous():
         raise ValueError("slot_map must be a contiguous int64 tensor on the pool's device with an entry per token")
     if D % 8:
@@ -244,10 +244,16 @@ def append_paged_kv_slots(pool: torch.Tensor, layer: int, k: torch.Tensor, v: to
     _lib.on_device(_lib.lib().subspec_kv_append_slots, a, dev, "subspec_kv_append_slots")
 
 
+def _lengths(t: torch.Tensor, dev: int, n: int, what: str) -> int:
+    if t.dtype != torch.int32 or t.get_device() != dev or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 [{n}] tensor on the pool's device")
+    return t.data_ptr()
+
+
 def _status_ptr(status: Optional[torch.Tensor], dev) -> int:
     if status is None:
         return 0
-    if status.dtype != torch.int32 or status.device != dev or status.numel() < 1:
+    if status.dtype != torch.int32 or status.get_device() != dev or status.numel() < 1:
         raise ValueError("status must be an int32 tensor on the pool's device")
     return status.data_ptr()
 
@@ -266,34 +272,34 @@ def _chunk_scratch_bytes(B, T, max_q_len, HQ, H, D, page_len, width, window, sin
 def _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, window, sinks, sm_scale, status,
                      out) -> torch.Tensor:
     L, P, _, page_len, H, D = _check_pool(pool, layer)
-    shape, dev = q.shape, pool.device
-    if len(shape) != 3 or q.dtype != pool.dtype or q.device != dev or shape[2] != D or D not in (64, 128):
+    shape, dtype, dev = q.shape, pool.dtype, pool.get_device()
+    if len(shape) != 3 or q.dtype != dtype or q.get_device() != dev or shape[2] != D or D not in (64, 128):
         raise ValueError("q must be [tokens, q_heads, head_dim] of the pool's type and head_dim (64 or 128) on its device")
     T, HQ, _ = shape
     if HQ < 1 or HQ % H:
         raise ValueError("q_heads must be a multiple of the pool's kv_heads")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous() or page_table.device != dev:
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or not page_table.is_contiguous() or page_table.get_device() != dev:
         raise ValueError("page_table must be a contiguous int32 [batch, pages_per_seq] tensor on the pool's device")
     B, width = page_table.shape
     if out is None:
-        out = torch.empty(T, HQ, D, dtype=q.dtype, device=dev)
-    elif out.dtype != q.dtype or out.shape != shape or out.device != dev or not (T == 0 or _aligned(out)):
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    elif out.dtype != dtype or out.shape != shape or out.get_device() != dev or not (T == 0 or _aligned(out)):
         raise ValueError("out must be a tensor of q's type and shape on q's device, its rows 16-byte aligned")
     elif T and out.data_ptr() == q.data_ptr():
         raise ValueError("out must not be q itself")
     max_q_len = T if max_q_len is None else int(max_q_len)
     if max_q_len < 0:
         raise ValueError("max_q_len must not be negative")
-    kv_ptr, indptr_ptr = _i32(kv_len, dev, B, "kv_len"), _i32(q_indptr, dev, B + 1, "q_indptr")
+    kv_ptr, indptr_ptr = _lengths(kv_len, dev, B, "kv_len"), _lengths(q_indptr, dev, B + 1, "q_indptr")
     if T == 0 or B == 0:
         return out
     if not _aligned(q):
         q = q.detach().clone(memory_format=torch.contiguous_format)
     max_q_len = min(max_q_len, T)
     need = _chunk_scratch_bytes(B, T, max_q_len, HQ, H, D, page_len, width, window, sinks)
-    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    scratch = pool.new_empty(need, dtype=torch.uint8) if need else None
     a = _lib.ChunkAttnArgs(C.sizeof(_lib.ChunkAttnArgs), B, T, max_q_len, HQ, H, D, layer, L, P, page_len, width,
-                           _lib.BF16 if q.dtype == torch.bfloat16 else _lib.F16, window, sinks, 0,
+                           _lib.BF16 if dtype == torch.bfloat16 else _lib.F16, window, sinks, 0,
                            pool.data_ptr(), page_table.data_ptr(), kv_ptr, indptr_ptr, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
                            1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
                            _status_ptr(status, dev), 0 if scratch is None else scratch.data_ptr(), need)

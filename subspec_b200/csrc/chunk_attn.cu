@@ -266,8 +266,7 @@ struct Pieces {
 
 template <bool kHalf, int kDim>
 __global__ void __launch_bounds__(kChunkThreads, 1)
-    chunk_attn_tc_kernel(const ChunkArgs ka, const __grid_constant__ CUtensorMap tmap_k,
-                         const __grid_constant__ CUtensorMap tmap_v) {
+    chunk_attn_tc_kernel(const ChunkArgs ka, const __grid_constant__ CUtensorMap tmap) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full[kRing], empty[kRing], s_ready[2], p_ready[2], o_done[2], my_turn[2], q_ready[2], fix, drained[2], pc_full[kPieces], pc_empty[kPieces];
   __shared__ union {
@@ -758,7 +757,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     } else {
       // ================= K (warp 18) and V (warp 19) tiles =================
       const int is_v = warp - kLoadWarp;
-      const CUtensorMap* map = is_v ? &tmap_v : &tmap_k;
       const int box = ka.box_rows, boxes = box > 0 ? kTileKeys / box : 0;
       const int chunk = lane % (kDim / 8), sub = lane / (kDim / 8);  // row-by-row copies
       constexpr int kRowsPerPass = 32 / (kDim / 8);
@@ -820,12 +818,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               const int kpos = t0 + lane * box;
               int unit = ka.units, slot = 0;  // outside the tensor: zeros, no memory is touched
               if (page >= 0 && page < a.num_pages) {
-                unit = page * ka.page_units + head;
+                unit = page * ka.page_units + (is_v ? ka.page_units / 2 : 0) + head;
                 slot = ka.page_shift >= 0 ? kpos & (a.page_len - 1) : kpos % a.page_len;
               } else if (page != -2) {
                 flag(a.dev_status, SUBSPEC_DEV_BAD_PAGE);
               }
-              tma_load_5d(dst + (size_t)lane * box * kDim * 2, map, slot >> 3, unit, bar);
+              tma_load_5d(dst + (size_t)lane * box * kDim * 2, &tmap, slot >> 3, unit, bar);
             }
             if (tail) {
               if (!(live = tc_wait(&fix, fixes++ & 1u, abort_flag))) break;
@@ -1019,45 +1017,40 @@ extern "C" int subspec_chunk_attention_scratch_bytes(const subspec_chunk_attn_ar
   return SUBSPEC_OK;
 }
 
-// The K (or V) rows of a layer as the copies see them: (64 dims | row of a group of 8 | half of the head's dims | group
-// of 8 rows in the page | unit), a unit being one row of one head: pages and heads both are whole numbers of units
-// apart, so the outermost coordinate addresses (page, head) at once and a box = a page's rows (or box_rows of them)
+// The rows of a layer as the copies see them: (64 dims | row of a group of 8 | half of the head's dims | group of 8 rows in
+// the page | unit), a unit being one row of one head: pages, their K and V rows and heads all are whole numbers of units
+// apart, so the outermost coordinate addresses (page, K or V, head) at once and a box = a page's rows (or box_rows of them)
 // of one head, landing group by group, half by half.
-static bool chunk_tensor_map(CUtensorMap* m, const ChunkArgs& ka, const unsigned char* base) {
+void subspec::chunk_tensor_map(ChunkArgs& ka, int rows, CUtensorMap* map) {
   const subspec_chunk_attn_args& a = ka.a;
+  memset(map, 0, sizeof(*map));
+  int box_rows = rows;
+  while (box_rows > 1 && a.page_len % box_rows) box_rows /= 2;  // the largest power of two up to a tile that divides a page
+  ka.box_rows = box_rows >= 8 && tensor_map_encoder() ? box_rows : 0;
+  if (!ka.box_rows) return;
   const cuuint64_t halves = a.head_dim / 64;
   const cuuint64_t dims[5] = {64, 8, halves, (cuuint64_t)a.page_len / 8, (cuuint64_t)ka.units};
   const cuuint64_t strides[4] = {(cuuint64_t)ka.row_stride, 128, (cuuint64_t)ka.row_stride * 8, (cuuint64_t)a.head_dim * 2};
-  const cuuint32_t box[5] = {64, 8, (cuuint32_t)halves, (cuuint32_t)ka.box_rows / 8, 1}, estr[5] = {1, 1, 1, 1, 1};
-  return tensor_map_encoder()(m, a.dtype == SUBSPEC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
-                              const_cast<unsigned char*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint32_t box[5] = {64, 8, (cuuint32_t)halves, (cuuint32_t)box_rows / 8, 1}, estr[5] = {1, 1, 1, 1, 1};
+  if (tensor_map_encoder()(map, a.dtype == SUBSPEC_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
+                           const_cast<unsigned char*>(ka.k_base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    ka.box_rows = 0;
 }
-
-namespace subspec {
-void chunk_tensor_maps(ChunkArgs& ka, int rows, CUtensorMap* k, CUtensorMap* v) {
-  memset(k, 0, sizeof(*k));
-  memset(v, 0, sizeof(*v));
-  int box = rows;
-  while (box > 1 && ka.a.page_len % box) box /= 2;  // the largest power of two up to a tile that divides a page
-  ka.box_rows = box >= 8 && tensor_map_encoder() ? box : 0;
-  if (ka.box_rows && !(chunk_tensor_map(k, ka, ka.k_base) && chunk_tensor_map(v, ka, ka.v_base))) ka.box_rows = 0;
-}
-}  // namespace subspec
 
 template <bool kHalf, int kDim>
 static int launch_chunk(ChunkArgs& ka, cudaStream_t stream) {
   const int rc = allow_smem<chunk_attn_tc_kernel<kHalf, kDim>>(tc_smem<kDim>());
   if (rc) return rc;
-  CUtensorMap tmap_k, tmap_v;
-  chunk_tensor_maps(ka, kTileKeys, &tmap_k, &tmap_v);
+  CUtensorMap tmap;
+  chunk_tensor_map(ka, kTileKeys, &tmap);
   int launched;
   if (ka.few_rows) {
     launched = launch_dependent(chunk_attn_tc_kernel<kHalf, kDim>, dim3((unsigned)ka.ctas), dim3(kChunkThreads), tc_smem<kDim>(),
-                                stream, ka, tmap_k, tmap_v);
+                                stream, ka, tmap);
   } else {
-    chunk_attn_tc_kernel<kHalf, kDim><<<ka.ctas, kChunkThreads, tc_smem<kDim>(), stream>>>(ka, tmap_k, tmap_v);
+    chunk_attn_tc_kernel<kHalf, kDim><<<ka.ctas, kChunkThreads, tc_smem<kDim>(), stream>>>(ka, tmap);
     launched = cuda_check(cudaGetLastError());
   }
   if (launched) return launched;
@@ -1090,7 +1083,7 @@ extern "C" int subspec_chunk_attention_paged(const subspec_chunk_attn_args* args
   ka.k_base = reinterpret_cast<const unsigned char*>(a.pool) + (size_t)a.layer * a.num_pages * ka.page_stride;
   ka.v_base = ka.k_base + a.page_len * ka.row_stride;
   ka.page_units = 2 * a.page_len * a.num_kv_heads;
-  const long long units = (long long)(a.num_pages - 1) * ka.page_units + a.num_kv_heads;
+  const long long units = (long long)(a.num_pages - 1) * ka.page_units + ka.page_units / 2 + a.num_kv_heads;
   if (units > 0x7fffffffLL) return SUBSPEC_EUNSUPPORTED;
   ka.units = (int)units;
   const size_t need = chunk_scratch_bytes(ka);

@@ -20,7 +20,7 @@ struct ChunkArgs {
   const unsigned char* k_base;
   const unsigned char* v_base;
   long long page_stride, row_stride;
-  int page_units, units;  // a page, and the whole layer, in rows of one head (the tensor maps' outermost coordinate)
+  int page_units, units;  // a page, and the whole layer, in rows of one head (the tensor map's outermost coordinate)
   int ctas;               // of the kernel for many rows (0: not launched)
   int4* runs;             // its runs: request, KV head, row tile of the first piece; 1: begun in an earlier run, 2: ends in this
   float* part_o;          // [run][2][256][head_dim] unnormalised rows: [0] of a row tile begun earlier, [1] of one that goes on
@@ -148,7 +148,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return d;
 }
 
-// One page's rows of one head: coordinates (dim, row of 8, half, group of 8 rows, unit), see chunk_tensor_map.
+// One page's rows of one head: coordinates (dim, row of 8, half, group of 8 rows, unit), see chunk_tensor_map (the last: V rows lie half a page behind K rows).
 __device__ __forceinline__ void tma_load_5d(void* dst_smem, const CUtensorMap* map, int c3, int c4, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3, %4}], [%5];" ::"r"(

@@ -92,8 +92,7 @@ struct Cursor {
 
 template <bool kHalf, int kDim, int kMT>
 __global__ void __launch_bounds__(kFewThreads, kFewPerSm)
-    chunk_attn_few_kernel(const ChunkArgs ka, const __grid_constant__ CUtensorMap tmap_k,
-                          const __grid_constant__ CUtensorMap tmap_v) {
+    chunk_attn_few_kernel(const ChunkArgs ka, const __grid_constant__ CUtensorMap tmap) {
   extern __shared__ unsigned char smem_raw[];
   constexpr int kStages = few_stages<kDim>(), kStageBytes = few_stage_bytes<kDim>(), kPlane = kStageBytes / 2;
   constexpr int kHalves = kDim / 64, kGroupBytes = 1024 * kHalves;
@@ -190,12 +189,12 @@ __global__ void __launch_bounds__(kFewThreads, kFewPerSm)
         const int kpos = t0 + copy_box * box;
         int unit = ka.units, slot = 0;  // outside the tensor: zeros, no memory is touched
         if (page >= 0 && page < a.num_pages) {
-          unit = page * ka.page_units + put.h;
+          unit = page * ka.page_units + (copy_v ? ka.page_units / 2 : 0) + put.h;
           slot = ka.page_shift >= 0 ? kpos & (a.page_len - 1) : kpos % a.page_len;
         } else if (page != -2) {
           flag(a.dev_status, SUBSPEC_DEV_BAD_PAGE);
         }
-        tma_load_5d(dst + (copy_v ? kPlane : 0) + copy_box * box * kDim * 2, copy_v ? &tmap_v : &tmap_k, slot >> 3, unit,
+        tma_load_5d(dst + (copy_v ? kPlane : 0) + copy_box * box * kDim * 2, &tmap, slot >> 3, unit,
                     &full[warp][s]);
       }
     } else {  // page lengths that are no multiple of 8: 16-byte copies, row by row
@@ -523,9 +522,9 @@ template <bool kHalf, int kDim, int kMT>
 int launch(ChunkArgs& ka, cudaStream_t stream) {
   const int rc = allow_smem<chunk_attn_few_kernel<kHalf, kDim, kMT>>(few_smem<kDim>());
   if (rc) return rc;
-  CUtensorMap tmap_k, tmap_v;
-  chunk_tensor_maps(ka, kWarpKeys, &tmap_k, &tmap_v);
-  chunk_attn_few_kernel<kHalf, kDim, kMT><<<kFewCtas, kFewThreads, few_smem<kDim>(), stream>>>(ka, tmap_k, tmap_v);
+  CUtensorMap tmap;
+  chunk_tensor_map(ka, kWarpKeys, &tmap);
+  chunk_attn_few_kernel<kHalf, kDim, kMT><<<kFewCtas, kFewThreads, few_smem<kDim>(), stream>>>(ka, tmap);
   const int launched = cuda_check(cudaGetLastError());
   if (launched) return launched;
   const long long rows = (long long)ka.a.max_q_len * ka.group;

@@ -129,7 +129,7 @@ class DevicePagePool:
             self.free_mask.data_ptr(), self.page_table.data_ptr(), self.n_pages.data_ptr(), self.kv_len.data_ptr(),
             self.kv_last_page_len.data_ptr(), set_ptr, n_new.data_ptr(), self.seq_indptr.data_ptr(),
             self.slot_map.data_ptr(), self.positions.data_ptr(), self.batch_indices.data_ptr(), self.status.data_ptr())
-        _lib.on_device(_lib.lib().subspec_chunk_plan, a, self.device, "subspec_chunk_plan")
+        _lib.on_device(_lib.lib().subspec_chunk_plan, a, self.slot_map.get_device(), "subspec_chunk_plan")
         return ChunkPlan(q_indptr=self.seq_indptr, slot_map=self.slot_map, positions=self.positions,
                          batch_indices=self.batch_indices, page_table=self.page_table, kv_len=self.kv_len)
 
