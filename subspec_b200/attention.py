@@ -7,6 +7,10 @@ under a custom mask.  Here both are kernels of the C-ABI library (`subspec_kv_ap
 `subspec_tree_attention_paged`) that take the pool, the page table and the mask as the other kernels of this
 package leave them: `KvCachePool.cache_data`, `DevicePagePool.page_table` / `kv_len`, and the
 [rows, prefix + tree columns] mask `DraftTreeBatch.finalize` writes.
+
+Prompts, decode steps and mixtures of them come as packed tokens of many requests (`DevicePagePool.plan_chunks`):
+`append_paged_kv_slots`, `chunk_attention_paged` (causal) and `window_attention_paged` (a sliding window whose first
+rows stay visible).
 """
 from __future__ import annotations
 
@@ -287,6 +291,8 @@ def _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, wi
         raise ValueError("out must be a tensor of q's type and shape on q's device, its rows 16-byte aligned")
     elif T and out.data_ptr() == q.data_ptr():
         raise ValueError("out must not be q itself")
+    elif T > 1 and out.stride(0) == 0 or HQ > 1 and out.stride(1) == 0:
+        raise ValueError("rows of out must not share memory")
     max_q_len = T if max_q_len is None else int(max_q_len)
     if max_q_len < 0:
         raise ValueError("max_q_len must not be negative")
@@ -300,7 +306,8 @@ def _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, wi
     scratch = pool.new_empty(need, dtype=torch.uint8) if need else None
     a = _lib.ChunkAttnArgs(C.sizeof(_lib.ChunkAttnArgs), B, T, max_q_len, HQ, H, D, layer, L, P, page_len, width,
                            _lib.BF16 if dtype == torch.bfloat16 else _lib.F16, window, sinks, 0,
-                           pool.data_ptr(), page_table.data_ptr(), kv_ptr, indptr_ptr, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+                           pool.data_ptr(), page_table.data_ptr(), kv_ptr, indptr_ptr, q.data_ptr(), q.stride(0),
+                           q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
                            1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale),
                            _status_ptr(status, dev), 0 if scratch is None else scratch.data_ptr(), need)
     _lib.on_device(_lib.lib().subspec_chunk_attention_paged, a, dev, "subspec_chunk_attention_paged")
@@ -327,8 +334,7 @@ def chunk_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, pa
 def window_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, page_table: torch.Tensor,
                            kv_len: torch.Tensor, q_indptr: torch.Tensor, window: int, sinks: int = 0,
                            max_q_len: Optional[int] = None, sm_scale: Optional[float] = None,
-                           status: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
-                           kv_splits: Optional[int] = None) -> torch.Tensor:
+                           status: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """`chunk_attention_paged` under a sliding window: a token at row p sees the `window` rows up to its own and the
     first `sinks` rows of the request.  Pages that lie outside every token's view are not read: they may have been given
     back (page_table entry -1)."""

@@ -48,6 +48,13 @@ def test_attention_refusals(bad):
         _call(**bad)
 
 
+@pytest.mark.parametrize("out", [torch.zeros(1, 4, 64, dtype=torch.bfloat16).expand(3, 4, 64),
+                                 torch.zeros(3, 1, 64, dtype=torch.bfloat16).expand(3, 4, 64)])
+def test_output_rows_that_share_memory_are_refused(out):
+    with pytest.raises(ValueError, match="share memory"):  # by its words: host tensors are refused in the end anyway
+        _call(out=out)
+
+
 @pytest.mark.parametrize("bad", [dict(window=0), dict(window=-3), dict(window=4, sinks=-1)])
 def test_window_refusals(bad):
     with pytest.raises(ValueError):
