@@ -42,7 +42,7 @@ namespace {
 //               warp 18 also walks the run and hands out its pieces.
 //
 // What it measured (B200, bf16, 28 query heads on 4 KV heads of 128 dims): 2048 tokens behind 30720 rows 745 us =
-// 1251 TFLOP/s, 0.75 of the card's cuBLAS burst (1.08 PFLOP/s at the 1 kW power cap when it runs for seconds).  A tile takes
+// 1251 TFLOP/s, 0.75 of the card's cuBLAS burst (861 to 869 us = 1.08 PFLOP/s at the power cap, 1.63 GHz, when it runs for seconds).  A tile takes
 // 2058 cycles of MMAs for both blocks and about 3600 in all.  Steps on the way, same case: an issuer per block without
 // turns 1306 us (both blocks in their softmax at once); one issuer 1015; runs over all SMs instead of a CTA per row tile,
 // half a tile of scores in registers instead of spilling, turns 790; two warps per row 756; Q rows by neighbouring lanes

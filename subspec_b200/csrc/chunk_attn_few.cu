@@ -14,8 +14,8 @@
 // (m, l, O) are joined in shared memory; a piece that is all of its (request, head) is divided and written, any other
 // goes to scratch, and a second kernel joins those.
 //
-// Measured (B200, 28 query heads on 4 KV heads of 128 dims, bf16): 64 single tokens behind 4k to 8k rows 119 us for
-// 714 MB = 6.0 TB/s, 0.91 of the card's copy; with the join and its launch 127 us.  A lone token behind 4095 rows, 15 us:
+// Measured (B200, 28 query heads on 4 KV heads of 128 dims, bf16): 64 single tokens behind 4k to 8k rows 120 us for
+// 714 MB = 5.95 TB/s, 0.91 of the card's copy; with the join and its launch 127 us.  A lone token behind 4095 rows, 15 us:
 // launch, lengths, page list, copies and join one after the other.  Two CTAs an SM with twice the stages are as fast
 // on long caches and slower on short pieces (48 windows of 1024 rows: 51.5 against 48.5 us); runs of at least 8 tiles
 // instead of 4 cost the lone token 3 us.

@@ -7,6 +7,7 @@ state in device arrays and brings it up to date with one kernel launch per step 
 include/subspec_b200.h): lengths set after a reorder, pages released, pages allocated for the next tree, and the
 flattened page-table tensors of the attention plan rebuilt -- nothing is read back.  The host classes in
 `subspec_b200.kv_cache` remain the drop-in mirror of the reference's interface; this is the batched form.
+`plan_chunks` does the same for chunks of any lengths and adds a slot and a position per token.
 """
 from __future__ import annotations
 
