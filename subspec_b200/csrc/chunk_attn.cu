@@ -217,6 +217,7 @@ struct Piece {
   int row0, rows;               // rows [row0, row0 + 256) of the request's
   int i0, ntiles, whole;        // cache tiles [i0, i0 + ntiles) of the row tile's list; all of them?
   int s_tiles, m0, hi, lo, snk;  // the list (TileList)
+  int last_seen[2];             // of the piece's tiles, the last one that a row of the block sees; -1: none
 };
 constexpr int kPieces = 4;  // in flight
 constexpr int kPieceReaders = kSoftmaxWarps + 3;
@@ -250,7 +251,7 @@ struct Pieces {
   }
   __device__ __forceinline__ Piece piece(bool any) const {
     return Piece{any, at.b, at.h, rq.q0, rq.first_pos, rq.kv_len, tile.row0, tile.rows, i0, ntiles, ntiles == tile.n,
-                 tile.list.s_tiles, tile.list.m0, tile.list.hi, tile.list.lo, tile.list.snk};
+                 tile.list.s_tiles, tile.list.m0, tile.list.hi, tile.list.lo, tile.list.snk, {-1, -1}};
   }
 
  private:
@@ -436,7 +437,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     // whether every row of the output begins on a sector
     const bool wide_out = !((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(2 * a.o_token_stride) | (uintptr_t)(2 * a.o_head_stride)) & 31u);
     bool live = true;
-    if (const Piece* first = peek()) {
+    // Q is handed over for the pieces that the block sees something of, and for no others: see the issuer's wait for it.
+    const Piece* first = peek();
+    if (first && first->last_seen[blk] >= 0) {
       load_q(*first);
       hand_q();
     }
@@ -578,6 +581,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       l = exchange(l, [](float x, float y) { return x + y; });
       // The block's Q has served its last scores: the next piece's comes while the last MMAs run.
       const Piece* following = live ? peek() : nullptr;
+      if (following && following->last_seen[blk] < 0) following = nullptr;
       if (following) load_q(*following);
       // ---- the result: O / l, or the part as it is ----
       if (live && done > 0) live = __all_sync(0xffffffffu, tc_wait(&o_done[blk], finished++ & 1u, abort_flag));
@@ -688,20 +692,24 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       auto next_entry = [&]() {
         if (++e == kRing) e = 0, ph ^= 1u;
       };
-      uint32_t seen = 0, piece = 0;
+      uint32_t seen = 0, queries = 0;
       bool issued = false;
-      for (; ok; ++piece) {
+      while (ok) {
         const Piece* now = peek();
         if (!now) break;
-        const int n = now->ntiles, i0 = now->i0, s_tiles = now->s_tiles, m0 = now->m0;
-        int bfirst, blast, last_seen = -1;
+        const int n = now->ntiles, i0 = now->i0, s_tiles = now->s_tiles, m0 = now->m0, last_seen = now->last_seen[blk];
+        int bfirst, blast;
         block_pos(*now, blk, bfirst, blast);
         pop();
         auto sees = [&](int i) { return block_sees(bfirst, blast, list_row(s_tiles, m0, i0 + i)); };
-        for (int i = n - 1; i >= 0 && last_seen < 0; --i)
-          if (sees(i)) last_seen = i;
         bool begun = false, sees_now = sees(0);
-        wait(&q_ready[blk], piece & 1u);
+        // One bit tells a phase of a barrier from the next, not from the one after it.  Nothing holds the softmax warps back
+        // in a piece of which their block sees nothing (a row tile of up to 128 rows has such a second block): they may be
+        // several pieces ahead of this warp.  So such pieces have no phase of q_ready.  Those that have one are at most one
+        // apart: the softmax hands over the next behind o_done of the one before, which this warp commits behind its own wait
+        // for that one's.  (The others: s_ready and p_ready answer each other, o_done is waited for before the p_ready that
+        // the next one needs, my_turn goes to and fro, a slot of the pieces is free when all readers have let go of it.)
+        if (last_seen >= 0) wait(&q_ready[blk], queries++ & 1u);
         wait(&full[e], ph);
         take_turn();
         if (elect_one()) {
@@ -777,8 +785,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           const bool any = walk.next(ka);
           now = walk.piece(any);
           if (!(live = tc_wait(&pc_empty[pc_slot], slot_ph, abort_flag))) break;
+          if (lane == 0) s_piece[pc_slot] = now;
+          __syncwarp();
+          if (any && lane < 2) {
+            int bfirst, blast, i = now.ntiles - 1;
+            block_pos(now, lane, bfirst, blast);
+            while (i >= 0 && blast >= 0 && !block_sees(bfirst, blast, list_row(now.s_tiles, now.m0, now.i0 + i))) --i;
+            s_piece[pc_slot].last_seen[lane] = blast >= 0 ? i : -1;
+          }
+          __syncwarp();
           if (lane == 0) {
-            s_piece[pc_slot] = now;
             mbar_arrive(&pc_full[pc_slot]);
             // what the join needs: the run's first row tile, whether it began in an earlier run, whether it ends in this
             if (first) *record = make_int4(now.b, now.h, walk.at.qt, any ? (now.i0 > 0 ? 1 : 0) | (now.i0 + now.ntiles == walk.tile.n ? 2 : 0) : 0);

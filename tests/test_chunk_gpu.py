@@ -595,3 +595,53 @@ def test_prompts_into_the_loop(cuda_lib):
     assert float((tree.float() - flat.view_as(tree).float()).abs().max()) <= 4 * 2 ** -8 * float(tree.float().abs().max())
     assert loop.status.item() == 0
     loop.pages.check_status()
+
+
+# ---------------------------------------------------------------- batches of many short chunks
+
+def _dense(q, k, v, window=0, sinks=0):
+    """`ao.chunk_attention` of finite rows with a dense mask (no loop over tokens)."""
+    n, HQ, D = q.shape
+    kv_len, G = k.shape[0], HQ // k.shape[1]
+    qd, kd, vd = q.double().transpose(0, 1), *(x.double().repeat_interleave(G, 1).transpose(0, 1) for x in (k, v))
+    p, j = torch.arange(kv_len - n, kv_len)[:, None], torch.arange(kv_len)[None, :]
+    see = j <= p
+    if window:
+        see &= (j > p - window) | (j < sinks)
+    w = torch.softmax((qd @ kd.transpose(1, 2) / D ** 0.5).masked_fill(~see, float("-inf")), -1)
+    return (w @ vd).transpose(0, 1), (w @ vd.abs()).transpose(0, 1)
+
+
+def _lengths(seed, count, lo, hi):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(lo, hi + 1, (count,), generator=g).tolist()
+
+
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16)])
+@pytest.mark.parametrize("new,cached,heads,kv_heads,window,sinks", [
+    ([5] * 3, [0] * 3, 8, 1, 0, 0),
+    ([20] * 3, [0] * 3, 4, 1, 0, 0),
+    ([5, 5, 30, 5, 5, 5, 40], [0] * 7, 8, 1, 0, 0),
+    ([20] * 64, [0] * 64, 32, 8, 0, 0),
+    (_lengths(31, 64, 1, 300), [0] * 64, 32, 8, 0, 0),
+    ([16] * 48, [100] * 48, 32, 8, 0, 0),
+    ([6] * 256, _lengths(32, 256, 30, 200), 28, 4, 0, 0),
+    (_lengths(33, 128, 8, 18), _lengths(34, 128, 0, 200), 28, 4, 0, 0),
+    ([16] * 64, [300] * 64, 32, 8, 100, 0),
+    (_lengths(35, 150, 3, 70), _lengths(36, 150, 0, 400), 8, 2, 60, 5),
+    ([17] * 300, [0] * 300, 16, 8, 0, 0),
+], ids=lambda x: None if isinstance(x, list) else str(x))
+def test_many_short_chunks(cuda_lib, new, cached, heads, kv_heads, window, sinks, D, dtype):
+    """Batches whose row tiles have up to 128 rows, the second block of a CTA none, one behind the other: every row
+    is written (the output starts as NaN), nothing is reported, the values are the formula's."""
+    c = _setup(37, new, cached, heads, kv_heads, D=D, dtype=dtype, layers=1, layer=0)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for kw in (dict(), dict(max_q_len=max(new))):
+        out = torch.full(c["q"].shape, float("nan"), dtype=dtype, device=DEV)
+        got = _run(c, window, sinks, status, out=out, **kw).double().cpu()
+        assert status.item() == 0
+        for b, n in enumerate(new):
+            lo = c["indptr"][b]
+            want, mag = _dense(c["q"][lo:lo + n], c["ks"][b], c["vs"][b], window, sinks)
+            err = (got[lo:lo + n] - want).abs()
+            assert bool((err <= _tolerance(want, mag, c["kv_len"][b], dtype, 6.0)).all()), b
