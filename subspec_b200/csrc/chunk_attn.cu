@@ -269,7 +269,8 @@ template <bool kHalf, int kDim>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     chunk_attn_tc_kernel(const ChunkArgs ka, const __grid_constant__ CUtensorMap tmap) {
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t full[kRing], empty[kRing], s_ready[2], p_ready[2], o_done[2], my_turn[2], q_ready[2], fix, drained[2], pc_full[kPieces], pc_empty[kPieces];
+  __shared__ __align__(8) uint64_t full[kRing], empty[kRing], s_ready[2], p_ready[2], o_done[2], my_turn[2], q_ready[2], fix, drained[2];
+  __shared__ __align__(8) uint64_t pc_full[kPieces], pc_empty[kPieces], pair_move[8];
   __shared__ union {
     long long cost[kGroups];  // of the groups of requests; then
     float row[kCtaRows];      // what the two warps of a row tell each other
@@ -319,9 +320,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       mbar_init(&pc_empty[k], kPieceReaders);
     }
     mbar_init(&fix, 1);
+    for (int k = 0; k < 8; ++k) {
+      mbar_init(&pair_move[k], 2);
+      s_move[k] = 0xffffffffu;
+    }
     mbar_init_fence();
     s_abort = 0;
-    for (int k = 0; k < 8; ++k) s_move[k] = 0xffffffffu;
   }
   __syncthreads();
   long long total = s_words.cost[lane] + s_words.cost[lane + 32];
@@ -353,12 +357,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const uint32_t tmem = s_tmem;
   volatile int* abort_flag = &s_abort;
 
+  // Every wait is bounded, and lanes may give up one by one: a warp goes on or leaves as a whole, with no lane behind at a
+  // vote or a warp barrier of the others.
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, tc_wait(bar, parity, abort_flag)) != 0; };
+
   // Reading the pieces: peek waits for the next one, pop lets go of its slot.
   int pc_slot = 0;
   uint32_t pc_phase = 0;
   auto peek = [&]() -> const Piece* {
-    const bool ok = __all_sync(0xffffffffu, tc_wait(&pc_full[pc_slot], pc_phase, abort_flag));
-    return ok && s_piece[pc_slot].valid ? &s_piece[pc_slot] : nullptr;
+    return warp_wait(&pc_full[pc_slot], pc_phase) && s_piece[pc_slot].valid ? &s_piece[pc_slot] : nullptr;
   };
   auto pop = [&]() {
     __syncwarp();
@@ -406,6 +413,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if (half == 1) word = x = join(x, word);
       pair_sync(pair);
       return half == 0 ? word : x;
+    };
+    // The named barriers of a pair have no limit: they stand only where both warps come whatever either of them gave up
+    // on, for reasons that both know.  Where one cannot tell whether the other comes, they meet at a barrier with one.
+    uint32_t moves = 0;
+    auto meet_to_move = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pair_move[pair - 1]);
+      return warp_wait(&pair_move[pair - 1], moves++ & 1u);
     };
     uint32_t seen = 0, finished = 0;  // tiles, and pieces with any, that this block has worked on
     // The warps of a block bring its rows of Q of a piece, sixteen each (rows that do not exist: zeros): neighbouring lanes
@@ -460,8 +475,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       for (int i = 0; i < ntiles; ++i) {
         const int t0 = list_row(s_tiles, m0, i0 + i);
         if (!block_sees(bfirst, blast, t0)) continue;
-        live = tc_wait(&s_ready[blk], seen & 1u, abort_flag);
-        __syncwarp();
+        live = warp_wait(&s_ready[blk], seen & 1u);
+        // (m is the same in both warps, so that both find the same here; once all rows have begun they stay so.)
+        const bool begins = !all_begun && __any_sync(0xffffffffu, m == -INFINITY);
+        if (begins) live = !pair_or(pair, !live);
+        if (!live && (begins || !kHalf)) break;  // (fp16: the pair meets below in every tile)
         tc_fence_after();
         const bool masked = !block_sees_all(bfirst, blast, t0);
         auto hide = [&](int c, uint32_t (&r)[32]) {
@@ -509,10 +527,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           all_begun = __all_sync(0xffffffffu, m != -INFINITY);
           rescale_o(alpha);
         };
-        if (!all_begun && __any_sync(0xffffffffu, m == -INFINITY)) move_to_max(false);
+        if (begins) move_to_max(false);
         if (!kHalf && s_move[pair - 1] == seen) {
           // 2^k past the reference point in sum: it moves up by k
-          const float both = exchange(l, [](float x, float y) { return x + y; });
+          if (half == 0) word = l;
+          if (!(live = meet_to_move())) break;
+          float both = l;
+          if (half == 1) word = both = l + word;
+          if (!(live = meet_to_move())) break;
+          if (half == 0) both = word;
           const int k = both > 1.f && both < kSpoilt ? (__float_as_int(both) >> 23) - 127 : 0;
           const float alpha = __int_as_float((127 - k) << 23);
           m += (float)k;
@@ -584,7 +607,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if (following && following->last_seen[blk] < 0) following = nullptr;
       if (following) load_q(*following);
       // ---- the result: O / l, or the part as it is ----
-      if (live && done > 0) live = __all_sync(0xffffffffu, tc_wait(&o_done[blk], finished++ & 1u, abort_flag));
+      if (live && done > 0) live = warp_wait(&o_done[blk], finished++ & 1u);
       if (following) hand_q();
       live = !pair_or(pair, !live);
       if (!live) break;
@@ -720,6 +743,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         pass_turn();
         issued = true;
         next_entry();
+        ok = __all_sync(0xffffffffu, ok);
         for (int i = 0; i < n && ok; ++i) {
           const int ve = e;
           const uint32_t vph = ph;
@@ -757,7 +781,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           ok = __all_sync(0xffffffffu, ok);
         }
       }
-      if (!ok && issued) {  // gave up: let the MMAs in flight finish before tensor memory is freed
+      if (issued) {  // whoever gave up: the MMAs in flight finish before tensor memory is freed
         if (elect_one()) tc_commit(&drained[blk]);
         __syncwarp();
         mbar_wait_bounded(&drained[blk], 0);
@@ -784,7 +808,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         } else {  // warp 18 walks the run and hands out its pieces
           const bool any = walk.next(ka);
           now = walk.piece(any);
-          if (!(live = tc_wait(&pc_empty[pc_slot], slot_ph, abort_flag))) break;
+          if (!(live = warp_wait(&pc_empty[pc_slot], slot_ph))) break;
           if (lane == 0) s_piece[pc_slot] = now;
           __syncwarp();
           if (any && lane < 2) {
@@ -819,7 +843,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         int page = page_of(0);
         for (int i = 0; i < ntiles; ++i) {
           const int next = page_of(i + 1);  // asked for a tile ahead: a trip to memory
-          if (!(live = tc_wait(&empty[e], ph, abort_flag))) break;
+          if (!(live = warp_wait(&empty[e], ph))) break;
           const int t0 = list_row(s_tiles, m0, i0 + i);
           unsigned char* dst = ring + (size_t)e * kTileBytes;
           if (boxes > 0) {
@@ -842,7 +866,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               tma_load_5d(dst + (size_t)lane * box * kDim * 2, &tmap, slot >> 3, unit, bar);
             }
             if (tail) {
-              if (!(live = tc_wait(&fix, fixes++ & 1u, abort_flag))) break;
+              if (!(live = warp_wait(&fix, fixes & 1u))) {
+                mbar_wait_bounded(&fix, fixes & 1u);  // this tile's copies land before the CTA leaves, too
+                break;
+              }
+              ++fixes;
               for (int x = lane; x < (z1 - z0) * (kDim / 8); x += 32) {
                 const int rr = z0 + x / (kDim / 8), c = x % (kDim / 8);
                 *reinterpret_cast<uint4*>(dst + (rr >> 3) * kGroupBytes + (c >> 3) * 1024 + (rr & 7) * 128 + ((c & 7) << 4)) =
