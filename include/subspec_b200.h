@@ -845,7 +845,8 @@ SUBSPEC_API int subspec_lm_head_verify(const subspec_lm_head_verify_args* args, 
 
 /* Block tables and slot maps from request lengths.  State as for
  * subspec_pages_update.  Per request: base = set_len ? set_len[b] : kv_len[b] rows are kept, pages behind them go
- * back to the pool (their page_table entries become -1), kv_len[b] = base + n_new[b], and missing pages are the
+ * back to the pool (their page_table entries become -1; entries that are -1 already, pages given back from behind a
+ * sliding window, are passed over, by subspec_pages_update too), kv_len[b] = base + n_new[b], and missing pages are the
  * lowest free ones, requests in batch order, all releases first.  q_indptr = the exclusive sum of n_new.  Token t:
  * batch_indices[t] = b, positions[t] = base + t - q_indptr[b], slot_map[t] = page * page_len + row.  The entries
  * from the last token to max_tokens become batch -1, position 0, slot -1, which the append skips.  Set in

@@ -337,7 +337,7 @@ def window_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, p
                            status: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """`chunk_attention_paged` under a sliding window: a token at row p sees the `window` rows up to its own and the
     first `sinks` rows of the request.  Pages that lie outside every token's view are not read: they may have been given
-    back (page_table entry -1)."""
+    back, that is, their page_table entries set to -1 and their bits in `DevicePagePool.free_mask` set."""
     window, sinks = int(window), int(sinks)
     if window < 1 or sinks < 0:
         raise ValueError("window must be at least 1 and sinks not negative")

@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kPlanThreads) chunk_plan_kernel(const subspec_
       const int pg = *entry;
       if (pg >= 0 && pg < a.num_pages)
         atomicOr(a.free_mask + (pg >> 5), 1u << (pg & 31));
-      else
+      else if (pg != -1)  // (-1: given back before, behind a sliding window)
         flag(a.dev_status, SUBSPEC_DEV_BAD_PAGE);
       *entry = -1;
     }

@@ -113,7 +113,8 @@ class DevicePagePool:
         stream (no synchronisation): `getKvCacheBatchPosition` for chunks of any lengths.
 
         `set_len[b]` (default `kv_len[b]`) rows are kept, the pages behind them go back to the pool and their entries
-        of `page_table` become -1; then kv_len[b] = set_len[b] + n_new[b], missing pages are the lowest free ones,
+        of `page_table` become -1 (entries that are -1 already, because the page was given back from behind a sliding
+        window, are passed over); then kv_len[b] = set_len[b] + n_new[b], missing pages are the lowest free ones,
         requests in batch order.  The plan's `slot_map` goes to `append_paged_kv_slots`, its `q_indptr`, `page_table`
         and `kv_len` to `chunk_attention_paged` / `window_attention_paged`; `max_append` of the constructor bounds the
         tokens of a step.  Running out of pages or of `max_append` is reported by `check_status`."""

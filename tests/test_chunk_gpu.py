@@ -645,3 +645,66 @@ def test_many_short_chunks(cuda_lib, new, cached, heads, kv_heads, window, sinks
             want, mag = _dense(c["q"][lo:lo + n], c["ks"][b], c["vs"][b], window, sinks)
             err = (got[lo:lo + n] - want).abs()
             assert bool((err <= _tolerance(want, mag, c["kv_len"][b], dtype, 6.0)).all()), b
+
+
+# ---------------------------------------------------------------- pages given back behind a window
+
+def _give_back(pages, b, first, last):
+    """Entries [first, last) of request b's list: -1 in the table, free in the mask."""
+    for j in range(first, last):
+        p = int(pages.page_table[b, j])
+        pages.page_table[b, j] = -1
+        pages.free_mask[p // 32] |= 1 << p % 32 if p % 32 < 31 else -2 ** 31  # (the words are signed)
+
+
+@pytest.mark.parametrize("release", ["plan", "update", "cut"])
+def test_requests_that_gave_pages_back_go_on_and_finish(cuda_lib, release):
+    """Plan, give back the pages behind the window, plan more tokens (which get those pages), attend, finish: nothing
+    is reported, no page is lost.  A page id outside the pool is reported as before."""
+    H, HQ, D, page_len, P = 2, 4, 64, 16, 70
+    g = torch.Generator().manual_seed(41)
+    pages = DevicePagePool(2, P, page_len, 64, DEV, max_append=700)
+    pool = torch.full((1, P, 2, page_len, H, D), float("nan"), dtype=torch.float16, device=DEV)
+    ks, vs = [torch.zeros(0, H, D)] * 2, [torch.zeros(0, H, D)] * 2
+
+    def step(new, window, sinks):
+        plan = pages.plan_chunks(_i32(new))
+        q, k, v = (torch.randn(sum(new), h, D, generator=g).to(torch.float16) for h in (HQ, H, H))
+        append_paged_kv_slots(pool, 0, k.to(DEV), v.to(DEV), slot_map=plan.slot_map)
+        status = torch.zeros(1, dtype=torch.int32, device=DEV)
+        out = window_attention_paged(q.to(DEV), pool, 0, page_table=plan.page_table, kv_len=plan.kv_len,
+                                     q_indptr=plan.q_indptr, window=window, sinks=sinks, status=status)
+        assert status.item() == 0
+        lo = 0
+        for b, n in enumerate(new):
+            ks[b], vs[b] = torch.cat([ks[b], k[lo:lo + n].float()]), torch.cat([vs[b], v[lo:lo + n].float()])
+            want, mag = _dense(q[lo:lo + n], ks[b], vs[b], window, sinks)
+            err = (out[lo:lo + n].double().cpu() - want).abs()
+            assert bool((err <= _tolerance(want, mag, len(ks[b]), torch.float16, 6.0)).all())
+            lo += n
+
+    step([600, 40], 100, 5)                      # 38 and 3 pages
+    assert pages.num_free_pages() == P - 41
+    _give_back(pages, 0, 1, 31)                  # rows 16 .. 495; the next token's window begins at row 501
+    assert pages.num_free_pages() == P - 11
+    step([20, 500], 100, 5)                      # the second request takes pages that the first gave back
+    assert pages.n_pages.tolist() == [39, 34] and set(pages.page_table[1, 3:34].tolist()) & set(range(1, 31))
+    pages.check_status()
+    if release == "cut":                         # back into the part that is gone, then on to nothing
+        pages.plan_chunks(_i32([0, 0]), set_len=_i32([200, 10]))
+        assert pages.n_pages.tolist() == [13, 1] and pages.num_free_pages() == P - 2
+        pages.check_status()
+    if release == "update":
+        pages.update(set_len=_i32([0, 0]), mode="prefill")
+    else:
+        pages.plan_chunks(_i32([0, 0]), set_len=_i32([0, 0]))
+    pages.check_status()
+    assert pages.num_free_pages() == P and pages.n_pages.tolist() == [0, 0] and bool((pages.free_mask[:2] == -1).all())
+    for finish in (lambda: pages.update(set_len=_i32([0, 0]), mode="prefill"),
+                   lambda: pages.plan_chunks(_i32([0, 0]), set_len=_i32([0, 0]))):
+        pages.plan_chunks(_i32([40, 0]))
+        for bad in (P, -2):
+            pages.page_table[0, 1] = bad
+        finish()
+        with pytest.raises(ValueError, match="page"):
+            pages.check_status()
