@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewPerSm)
       }
       // 0 * inf from a V row that only other rows of the tile see, or scores of -inf alone: key by key
       uint32_t again = __ballot_sync(0xffffffffu, whole && grow < rows && odd && lsum == lsum && row_pos >= 0);
+      __syncwarp();  // what eight lanes wrote of such a row lies before what all 32 write over it
       while (again) {
         const int src = __ffs(again) - 1;
         again &= ~(0xffu << (src & ~7));  // the eight lanes of a row

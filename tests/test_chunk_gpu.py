@@ -708,3 +708,26 @@ def test_requests_that_gave_pages_back_go_on_and_finish(cuda_lib, release):
         finish()
         with pytest.raises(ValueError, match="page"):
             pages.check_status()
+
+
+@pytest.mark.parametrize("D,dtype,per", [(128, torch.bfloat16, 2), (64, torch.float16, 4), (128, torch.float16, 6)])
+def test_many_rows_done_over(cuda_lib, D, dtype, per):
+    """Short chunks whose last token's V row holds an infinity in every dim: all rows in front of it are written twice, by
+    the tile (0 * inf) and key by key.  The second writing is what stays, call after call."""
+    B, heads, kv_heads = 200, 8, 2
+    c = _setup(43, [per] * B, _lengths(44, B, 0, 60), heads, kv_heads, D=D, dtype=dtype)
+    for b in range(B):
+        j = c["kv_len"][b] - 1
+        c["vs"][b][j] = float("inf")
+        c["pool"][1, c["table"][b, j // 16], 1, j % 16] = float("inf")
+    first = None
+    for _ in range(20):
+        got = _run(c, max_q_len=per)
+        assert first is None or torch.equal(got, first)
+        first = got
+    got = first.view(B, per, heads, D).double().cpu()
+    assert bool((got[:, -1] == float("inf")).all())
+    for b in range(B):
+        q = c["q"][b * per:(b + 1) * per - 1]
+        want, mag = _dense(q, c["ks"][b][:-1], c["vs"][b][:-1])
+        assert bool(((got[b, :-1] - want).abs() <= _tolerance(want, mag, c["kv_len"][b], dtype, 6.0)).all()), b
