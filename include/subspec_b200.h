@@ -76,6 +76,9 @@ typedef void* subspec_stream_t; /* a cudaStream_t; NULL = legacy default stream 
 SUBSPEC_API const char* subspec_version(void);
 /* cudaGetErrorString of the last CUDA error an entry point saw on this thread */
 SUBSPEC_API const char* subspec_last_cuda_error(void);
+/* A status word of the current device that belongs to the library: zero at load, for `dev_status` of callers that keep
+ * none of their own.  Kernels OR bits into it; whoever reads it clears it.  The address holds as long as the library. */
+SUBSPEC_API int subspec_default_status(uint32_t** word);
 
 /* ------------------------------------------------------------------------
  * Tree verify + accept, one launch per batch of independent sequences.

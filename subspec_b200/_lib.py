@@ -266,6 +266,7 @@ SYMBOLS = {
     "subspec_pages_update": (C.c_int, [C.POINTER(PagesArgs), _vp]),
     "subspec_tree_attention_paged": (C.c_int, [C.POINTER(TreeAttnArgs), _vp]),
     "subspec_kv_append_paged": (C.c_int, [C.POINTER(KvAppendArgs), _vp]),
+    "subspec_default_status": (C.c_int, [C.POINTER(_vp)]),
     "subspec_chunk_plan": (C.c_int, [C.POINTER(ChunkPlanArgs), _vp]),
     "subspec_kv_append_slots": (C.c_int, [C.POINTER(KvAppendSlotsArgs), _vp]),
     "subspec_chunk_attention_scratch_bytes": (C.c_int, [C.POINTER(ChunkAttnArgs), C.POINTER(C.c_size_t)]),
@@ -334,6 +335,41 @@ def on_device(fn, args, index: int, what: str) -> None:
             rc = fn(C.byref(args), _raw_stream(index))
     if rc:
         check(rc, what)
+
+
+_default_status: dict = {}
+
+
+def default_status(index: int) -> int:
+    """Address of the library's own status word on device `index` (`subspec_default_status`)."""
+    word = _default_status.get(index)
+    if word is None:
+        import torch
+
+        at = _vp()
+        with torch.cuda.device(index):
+            check(lib().subspec_default_status(C.byref(at)), "subspec_default_status")
+        word = _default_status[index] = at.value
+    return word
+
+
+class _DeviceWord:
+    """What torch.as_tensor needs to see an int32 at a device address."""
+
+    def __init__(self, address: int):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False), "version": 2}
+
+
+def take_default_status(index: int) -> int:
+    """The word's bits, which it loses.  Synchronises with the current stream of the device."""
+    import torch
+
+    with torch.cuda.device(index):
+        word = torch.as_tensor(_DeviceWord(default_status(index)), device=f"cuda:{index}")
+        bits = int(word.item())
+        if bits:
+            word.zero_()
+    return bits
 
 
 _current_device = _raw_stream = None

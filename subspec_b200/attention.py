@@ -223,8 +223,8 @@ def append_paged_kv_slots(pool: torch.Tensor, layer: int, k: torch.Tensor, v: to
     """k, v [tokens, kv_heads, head_dim] of packed requests -> rows `slot_map[t]` of layer `layer`.
 
     `slot_map` int64 [>= tokens] as `DevicePagePool.plan_chunks` leaves it: page * page_len + row, all different;
-    negative ones are skipped (a padded batch), one past the pool sets `status`.  k and v may be slices of a fused
-    projection."""
+    negative ones are skipped (a padded batch), one past the pool sets `status` (default: what `check_status` reads).  k
+    and v may be slices of a fused projection."""
     L, P, _, page_len, H, D = _check_pool(pool, layer)
     shape, dtype, dev = k.shape, pool.dtype, pool.get_device()
     if len(shape) != 3 or shape != v.shape or shape[1] != H or shape[2] != D or k.dtype != dtype or \
@@ -256,10 +256,22 @@ def _lengths(t: torch.Tensor, dev: int, n: int, what: str) -> int:
 
 def _status_ptr(status: Optional[torch.Tensor], dev) -> int:
     if status is None:
-        return 0
+        return 0 if dev < 0 else _lib.default_status(dev)
     if status.dtype != torch.int32 or status.get_device() != dev or status.numel() < 1:
         raise ValueError("status must be an int32 tensor on the pool's device")
     return status.data_ptr()
+
+
+def check_status(device=None) -> None:
+    """Raise for what the calls on packed tokens without a `status` of their own reported on `device` (default: the
+    current one) since the last check: bad lengths, pages and slots, a wait that ran out.  The output rows concerned may
+    never have been written.  Synchronises with the device's current stream."""
+    dev = torch.device("cuda" if device is None else device)
+    if dev.type != "cuda":
+        raise ValueError("the status word belongs to a CUDA device")
+    word = _lib.take_default_status(torch.cuda.current_device() if dev.index is None else dev.index)
+    if word:
+        raise ValueError("kernels over the paged cache: " + _lib.dev_status_text(word))
 
 
 @functools.lru_cache(maxsize=1024)
@@ -325,7 +337,8 @@ def chunk_attention_paged(q: torch.Tensor, pool: torch.Tensor, layer: int, *, pa
     (append first), and each sees the rows up to its own.  One token (a decode step) to whole prompts, mixed at will.
     `max_q_len`: no request brings more (default: all the tokens) -- give it where it is known, the kernels for a few
     rows per request are chosen by it.  Rows of the output behind q_indptr[-1] are left as they were; what a token does
-    not see has no influence on it, infinities and NaN included.  `out` must not overlap q.  Requests may share pages
+    not see has no influence on it, infinities and NaN included.  What is wrong on the device (lengths, pages, more tokens
+    than `max_q_len`) sets `status`, an int32 tensor, by default a word that `check_status` reads.  `out` must not overlap q.  Requests may share pages
     (a common prefix).  What `DevicePagePool.plan_chunks` returned fits as
     it is: chunk_attention_paged(q, pool, layer, page_table=plan.page_table, kv_len=plan.kv_len, q_indptr=plan.q_indptr)."""
     return _chunk_attention(q, pool, layer, page_table, kv_len, q_indptr, max_q_len, 0, 0, sm_scale, status, out)

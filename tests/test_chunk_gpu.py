@@ -731,3 +731,49 @@ def test_many_rows_done_over(cuda_lib, D, dtype, per):
         q = c["q"][b * per:(b + 1) * per - 1]
         want, mag = _dense(q, c["ks"][b][:-1], c["vs"][b][:-1])
         assert bool(((got[b, :-1] - want).abs() <= _tolerance(want, mag, c["kv_len"][b], dtype, 6.0)).all()), b
+
+
+# ---------------------------------------------------------------- errors without a status word of the caller's
+
+def test_errors_without_a_status_are_kept(cuda_lib):
+    """Calls that leave `status` out report to the library's word of the device, eager and captured, which check_status
+    reads and clears; calls that bring a word of their own leave it alone."""
+    from subspec_b200.attention import check_status
+
+    try:
+        check_status()  # (what an earlier test may have left)
+    except ValueError:
+        pass
+    for new in ([1, 1], [40, 40]):  # either kernel
+        c = _setup(51, new, [60, 60], 4, 2)
+        _run(c)
+        check_status()
+        good = c["table"].clone()
+        c["table"][0, 1] = 10 ** 6
+        own = torch.zeros(1, dtype=torch.int32, device=DEV)
+        _run(c, status=own)
+        check_status()
+        assert own.item() == 8
+        _check(c, _run(c), only=[1])
+        with pytest.raises(ValueError, match="page"):
+            check_status(DEV)
+        check_status(torch.device(DEV, 0))
+        c["table"] = good
+        _run(c, window=30, max_q_len=new[0] - 1 or 0)
+        if new[0] > 1:  # (max_q_len 0: nothing to do, nothing launched)
+            with pytest.raises(ValueError, match="count"):
+                check_status()
+        check_status()
+    pool = torch.zeros(1, 4, 2, 4, 2, 64, dtype=torch.bfloat16, device=DEV)
+    k = torch.zeros(2, 2, 64, dtype=torch.bfloat16, device=DEV)
+    slots = torch.tensor([0, 16], device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        append_paged_kv_slots(pool, 0, k, k, slot_map=slots)
+    check_status()
+    graph.replay()
+    with pytest.raises(ValueError, match="index"):
+        check_status()
+    slots.fill_(-1)
+    graph.replay()
+    check_status()

@@ -160,3 +160,11 @@ def test_argument_structs_match_the_header(tmp_path):
         assert int(got[cname]) == C.sizeof(mirror)
         for f, _ in mirror._fields_:
             assert int(got[f"{cname}.{f}"]) == getattr(mirror, f).offset, (cname, f)
+
+
+def test_the_status_word_belongs_to_a_device(cuda_lib):
+    from subspec_b200.attention import check_status
+
+    with pytest.raises(ValueError, match="CUDA"):
+        check_status("cpu")
+    assert cuda_lib.subspec_default_status(None) == _lib.EINVAL
