@@ -476,10 +476,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const int t0 = list_row(s_tiles, m0, i0 + i);
         if (!block_sees(bfirst, blast, t0)) continue;
         live = warp_wait(&s_ready[blk], seen & 1u);
-        // (m is the same in both warps, so that both find the same here; once all rows have begun they stay so.)
-        const bool begins = !all_begun && __any_sync(0xffffffffu, m == -INFINITY);
-        if (begins) live = !pair_or(pair, !live);
-        if (!live && (begins || !kHalf)) break;  // (fp16: the pair meets below in every tile)
         tc_fence_after();
         const bool masked = !block_sees_all(bfirst, blast, t0);
         auto hide = [&](int c, uint32_t (&r)[32]) {
@@ -527,7 +523,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           all_begun = __all_sync(0xffffffffu, m != -INFINITY);
           rescale_o(alpha);
         };
-        if (begins) move_to_max(false);
+        // (m is the same in both warps, so that both find the same here; once all rows have begun they stay so.)
+        if (!all_begun && __any_sync(0xffffffffu, m == -INFINITY)) {
+          live = !pair_or(pair, !live);
+          if (!live) break;
+          move_to_max(false);
+        } else if (!kHalf && !live) {
+          break;  // (fp16: the pair meets below in every tile)
+        }
         if (!kHalf && s_move[pair - 1] == seen) {
           // 2^k past the reference point in sum: it moves up by k
           if (half == 0) word = l;
