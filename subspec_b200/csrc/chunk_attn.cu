@@ -32,7 +32,10 @@ namespace {
 //
 //   warps 0-15  softmax, eight warps per block: thread = query row = lane of tensor memory, two warps per row, one for
 //               either half of a tile's 128 scores.  A thread writes P = 2^(S c - m) as 16-bit pairs over the first of the
-//               columns it read and sums P in fp32.  m, the reference point, is the maximum of the first tile, and moves
+//               columns it read and sums P in fp32.  (P is rounded to the cache's type because an MMA takes both operands
+//               in it: P in two 16-bit terms would be half as many MMAs again.  Half a step a weight; against 64 bits
+//               the output is off by 2.3e-3 of its norm in bf16 and 2.8e-4 in fp16, where rounding it alone makes 1.7e-3
+//               and 2.1e-4.)  m, the reference point, is the maximum of the first tile, and moves
 //               (the row of O in tensor memory is rescaled) only when the sums say that a later score has run far ahead of
 //               it.  They also bring the block's Q and write its output.
 //   warps 16, 17  issue the MMAs of a block each, in turns: O += P V (P from tensor memory, V MN-major as the cache has
@@ -41,12 +44,14 @@ namespace {
 //   warp 18     brings the K tiles, warp 19 the V tiles, into a ring of five entries, K(0), V(0), K(1), V(1), ...;
 //               warp 18 also walks the run and hands out its pieces.
 //
-// What it measured (B200, bf16, 28 query heads on 4 KV heads of 128 dims): 2048 tokens behind 30720 rows 745 us =
-// 1251 TFLOP/s, 0.75 of the card's cuBLAS burst (861 to 869 us = 1.08 PFLOP/s at the power cap, 1.63 GHz, when it runs for seconds).  A tile takes
-// 2058 cycles of MMAs for both blocks and about 3600 in all.  Steps on the way, same case: an issuer per block without
+// What it measured (B200, bf16, 28 query heads on 4 KV heads of 128 dims): 2048 tokens behind 30720 rows 870 us = 1.07
+// PFLOP/s call after call, at the power cap (1.64 GHz; on another card 896); a few calls alone 754 us = 1236 TFLOP/s, 0.74 of
+// the card's cuBLAS burst.  A tile takes 2058 cycles of MMAs for both blocks and about 3600 in all.  64 prompts of 30 to 60
+// tokens on 32/8 heads 44 us, 256 drafts of 3 to 6 tokens behind 50 to 200 rows 81 us (floors 9 and 13: one short row
+// tile after the other, 9 thousand cycles each).  Steps on the way, same case: an issuer per block without
 // turns 1306 us (both blocks in their softmax at once); one issuer 1015; runs over all SMs instead of a CTA per row tile,
 // half a tile of scores in registers instead of spilling, turns 790; two warps per row 756; Q rows by neighbouring lanes
-// and 32-byte stores 745.  Tried and no faster: separate score buffers for the tile's halves (S of 64 columns: MMAs 2484
+// and 32-byte stores 745; waits that leave no warp behind when one gives up 754.  Tried and no faster: separate score buffers for the tile's halves (S of 64 columns: MMAs 2484
 // cycles a tile) 740 to 850; a share of the exponentials as a polynomial on the FMA pipe 737 to 760.
 //
 // A tile lies in shared memory as 16 groups of 8 rows; a group as one (head_dim 64) or two halves of 64 dims, a half as
@@ -64,7 +69,9 @@ constexpr int kChunkThreads = 32 * (kSoftmaxWarps + 4);
 constexpr int kIssuerWarp = kSoftmaxWarps, kLoadWarp = kIssuerWarp + 2;
 constexpr uint32_t kBlockCols = 256, kOCol = 128;
 constexpr int kMinRun = 4;    // cost a run holds at least (its cache tiles and one for each row tile)
-constexpr int kSnapTiles = 8;  // row tiles of up to so many cache tiles are not cut where runs are long
+// Row tiles of up to so many cache tiles are not cut where runs are long.  (Measured at 0, 4, 8 and 16: six prompts 232, 233,
+// 235, 228 us, two windowed prompts 192, 192, 190, 186; short chunks, drafts and mixed batches alike within 2 %.)
+constexpr int kSnapTiles = 8;
 constexpr int kGroups = 64;    // groups of requests whose costs are summed up side by side
 
 template <int kDim>
@@ -334,6 +341,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   total *= a.num_kv_heads;
   const int runs = (int)max(1LL, min((long long)gridDim.x, total / kMinRun));
   // row tiles of up to so many cache tiles are not cut: a part costs about two tiles, an uneven run up to half the tile
+  // (a half or an eighth of the run instead of a quarter: the same within 2 %)
   const int snap = (int)min((long long)kSnapTiles, total / runs / 4);
   int4* record = ka.runs + run;
   if (total == 0 || run >= runs) {
@@ -1020,7 +1028,10 @@ static void chunk_sizes(ChunkArgs& ka) {
   ka.group = a.num_q_heads / a.num_kv_heads;
   // Which kernel a request's rows go to.  Up to 32 rows for every request: the kernel for few rows does it all.  More
   // for some: it still takes the requests of up to 16, where the token counts leave room for such beside the longest
-  // (on average at most 64 rows each).
+  // (on average at most 64 rows each).  Measured on 32 requests beside a chunk of 1024 tokens, 4 heads a group, with and
+  // without this kernel: 1 token each 134 and 138 us, 2 to 4 tokens 135 and 140; where it finds little or nothing to do its
+  // launch and join cost: 4 to 8 tokens 151 and 135, 8 to 16 tokens 148 and 138, 16 to 32 tokens 152 and 142 (it is left out).
+  // (A decode step that comes without max_q_len takes both kernels, too: 64 requests 137 us instead of 126.)
   const long long most = (long long)a.max_q_len * ka.group;
   const long long others = (long long)(a.tokens - a.max_q_len) * ka.group;
   ka.few_rows = most <= 16 ? 16 : most <= 32 ? 32 : a.batch > 1 && others <= 64LL * (a.batch - 1) ? 16 : 0;

@@ -19,6 +19,13 @@
 // launch, lengths, page list, copies and join one after the other.  Two CTAs an SM with twice the stages are as fast
 // on long caches and slower on short pieces (48 windows of 1024 rows: 51.5 against 48.5 us); runs of at least 8 tiles
 // instead of 4 cost the lone token 3 us.
+//
+// That is the variant of up to 16 rows.  The one of 17 to 32 keeps two row tiles of Q and O under the same bound of 168
+// registers and spills (head_dim 128: 932 bytes stored and 964 loaded, 64: 88 and 116): 64 requests of 2 to 4 tokens, 28
+// rows at most, behind 2k to 8k rows take 370 us where 1 or 2 tokens take 112 (floors 116 and 93).
+//
+// P is rounded to the cache's type, as in the tiles for many rows (chunk_attn.cu) and for the same reason.  Page lengths
+// that are no multiple of 8 are copied 16 bytes a lane: the 64 single tokens 303 us instead of 126 at pages of 20 rows.
 #include "chunk_attn.cuh"
 #include "chunk_attn_few.cuh"
 
