@@ -45,14 +45,16 @@ namespace {
 //               warp 18 also walks the run and hands out its pieces.
 //
 // What it measured (B200, bf16, 28 query heads on 4 KV heads of 128 dims): 2048 tokens behind 30720 rows 870 us = 1.07
-// PFLOP/s call after call, at the power cap (1.64 GHz; on another card 896); a few calls alone 754 us = 1236 TFLOP/s, 0.74 of
-// the card's cuBLAS burst.  A tile takes 2058 cycles of MMAs for both blocks and about 3600 in all.  64 prompts of 30 to 60
-// tokens on 32/8 heads 44 us, 256 drafts of 3 to 6 tokens behind 50 to 200 rows 81 us (floors 9 and 13: one short row
-// tile after the other, 9 thousand cycles each).  Steps on the way, same case: an issuer per block without
-// turns 1306 us (both blocks in their softmax at once); one issuer 1015; runs over all SMs instead of a CTA per row tile,
-// half a tile of scores in registers instead of spilling, turns 790; two warps per row 756; Q rows by neighbouring lanes
-// and 32-byte stores 745; waits that leave no warp behind when one gives up 754.  Tried and no faster: separate score buffers for the tile's halves (S of 64 columns: MMAs 2484
-// cycles a tile) 740 to 850; a share of the exponentials as a polynomial on the FMA pipe 737 to 760.
+// PFLOP/s call after call, at the power cap (1.64 GHz; on another card 896); a few calls alone 754 us = 1236 TFLOP/s, 0.74
+// of the card's cuBLAS burst.  A tile takes 2058 cycles of MMAs for both blocks and about 3600 in all.  64 prompts of 30
+// to 60 tokens on 32/8 heads 44 us, 256 drafts of 3 to 6 tokens behind 50 to 200 rows 81 us (floors 9 and 13; in a launch
+// list 45 and 74 for this kernel, which takes three or four, and seven, short row tiles one after the other, and 7 for a
+// join that finds nothing to do).  Steps on the way, same case: an issuer per block without turns 1306 us (both blocks in
+// their softmax at once); one issuer 1015; runs over all SMs instead of a CTA per row tile, half a tile of scores in
+// registers instead of spilling, turns 790; two warps per row 756; Q rows by neighbouring lanes and 32-byte stores 745;
+// waits that leave no warp behind when one gives up 754.  Tried and no faster: separate score buffers for the tile's
+// halves (S of 64 columns: MMAs 2484 cycles a tile) 740 to 850; a share of the exponentials as a polynomial on the FMA
+// pipe 737 to 760.
 //
 // A tile lies in shared memory as 16 groups of 8 rows; a group as one (head_dim 64) or two halves of 64 dims, a half as
 // 8 rows of 128 bytes under the 128-byte swizzle: the layout the tensor cores read either way round, in which the rows
